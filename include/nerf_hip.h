@@ -238,6 +238,45 @@ int nerf_linear_bwd_noalloc(const float* dy, int64_t lddy, const float* y, const
                             double pre, double post, const float* x, int64_t ldx, const float* W, int64_t M, int K, int N,
                             float* dx, int64_t lddx, float* dW, float* db, void* stream);
 
+/* ---- microscaled 4-bit (MXFP4) rows and products (no counterpart in the reference, which is fp32 throughout) ----
+ * Dense layers of any width on the 4-bit matrix pipe (v_mfma_scale_f32_16x16x128_f8f6f4), forward and backward, next to
+ * the layer-wise fp32 kernels above.  A row is cut into blocks of 32 values; a block holds one power-of-two scale
+ * 2^(s - 127), s = max(E - 2, 0) with E the biased fp32 exponent field of its largest magnitude, and 32 codes of 4 bits
+ * (sign, two exponent bits, one mantissa bit: 0 .5 1 1.5 2 3 4 6), each x / scale rounded to nearest, ties to even,
+ * saturated at 6.  A block with a NaN or an infinity gets s = 255 and reads back as NaN as a whole.
+ * Packed rows are back to back and padded to 128 values with zeros: codes [rows][64 ceil(K / 128)] bytes (low nibble = even
+ * index, 16-byte aligned), scales [rows][4 ceil(K / 128)] bytes (4-byte aligned); nerf_mx_codes_bytes /
+ * nerf_mx_scales_bytes give the sizes (0 for sizes the library does not take).
+ * Types of x, bias, y, dy and the gradients: NERF_F32, NERF_BF16 or NERF_F16, one per call; element pitches ldx, ldy ...
+ * may exceed the row length. */
+#define NERF_F32 0
+#define NERF_BF16 1
+#define NERF_F16 2
+size_t nerf_mx_codes_bytes(int64_t rows, int64_t K);
+size_t nerf_mx_scales_bytes(int64_t rows, int64_t K);
+int nerf_mx_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, void* stream);
+/* out[m][k] = code * scale, rounded once to the type (exact in fp32 and bf16). */
+int nerf_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, int dtype, void* out, int64_t ldo,
+                       void* stream);
+
+/* y[M,N] = post * f(pre * (Q(x) W^T + b)): x [M,K] is quantised by the call, W [N,K] comes packed, f = NERF_ACT_*, b [N] or
+ * NULL; sums in fp32.  For a backward pass the call also writes (NULL to skip): slope [M,N] fp32 = dy/dz for NERF_ACT_SIN
+ * and NERF_ACT_SIGMOID; mask [M][ceil(N / 16)] = the decisions of NERF_ACT_RELU, one bit each; xcodes, xscales = the
+ * quantised x.  workspace: nerf_mx_linear_fwd_workspace_bytes(M, K, N) bytes, 16-byte aligned. */
+size_t nerf_mx_linear_fwd_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales, const void* bias, int64_t M,
+                       int64_t K, int64_t N, int act, double pre, double post, void* y, int64_t ldy, float* slope, uint16_t* mask,
+                       uint8_t* xcodes, uint8_t* xscales, void* workspace, void* stream);
+
+/* Gradients of the product at the rounded operands (straight through the rounding): dz = dy * dy/dz, dx [M,K] = dz W,
+ * dW [N,K] = dz^T Q(x), db [N] = column sums of dz, each skipped where NULL.  slope / mask / xcodes / xscales: what the
+ * forward wrote.  bf16 matrix pipe, dz as up to three bf16 terms (fp32 accuracy for fp32), fp32 sums in a fixed order (no
+ * atomics).  workspace: nerf_mx_linear_bwd_workspace_bytes(...) bytes, 16-byte aligned. */
+size_t nerf_mx_linear_bwd_workspace_bytes(int dtype, int act, int64_t M, int64_t K, int64_t N, int need_dx, int need_dw, int need_db);
+int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const float* slope, const uint16_t* mask, int act, double pre, double post,
+                       const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes, const uint8_t* wscales, int64_t M, int64_t K,
+                       int64_t N, void* workspace, void* dx, int64_t lddx, void* dw, void* db, void* stream);
+
 /* ---- optimizer: torch.optim.Adam as train.py:123,182 uses it (no weight decay, no amsgrad) --
  * One launch over a flat parameter buffer: p, g, m, v [n].  step is 1-based. */
 int nerf_adam_step(float* p, const float* g, float* m, float* v, int64_t n, int step, double lr, double beta1,

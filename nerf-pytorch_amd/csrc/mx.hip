@@ -1,0 +1,192 @@
+// Microscaled 4-bit (MXFP4) rows: quantise and read back.  The format is described in mx_common.h.
+//
+// Both kernels are bound by HBM: a thread owns eight consecutive values (16 bytes of a 16-bit type, 32 of fp32), the four
+// threads of a quad one block.  The block's maximum takes two DPP steps, the rounding is the conversion instruction's
+// (v_cvt_scalef32_pk_fp4_f32: to nearest even, saturating).  Packed rows are back to back, so thread i writes code word i and
+// block i / 4's scale whatever the row's length; only the unpacked side needs the row, hence a division, and not even that
+// where rows are whole multiples of 128 values and back to back (FLAT).
+#include "mx_common.h"
+
+namespace mxk {
+namespace {
+
+// row of group i, in 32 bits wherever the count allows it (a 64-bit division is some hundred instructions)
+__device__ __forceinline__ int64_t row_of(int64_t i, int64_t total, int groups) {
+    return total <= 0xffffffffll ? (int64_t)((unsigned)i / (unsigned)groups) : i / groups;
+}
+
+constexpr int UNROLL = 4;   // groups of eight values per thread, all loads of a thread in flight together
+
+template <typename T, bool VEC, bool FLAT>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t total, int64_t K, int groups,
+                                                         unsigned* __restrict__ codes, uint8_t* __restrict__ scales) {
+    float v[UNROLL][8];
+    const int64_t base = (int64_t)blockIdx.x * (256 * UNROLL) + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const int64_t i = base + u * 256;
+        if (i < total) {
+            if constexpr (FLAT) {
+                load8(x + i * 8, v[u]);
+            } else {
+                const int64_t row = row_of(i, total, groups), k = (i - row * groups) * 8;
+                if (VEC && k + 8 <= K) load8(x + row * ldx + k, v[u]);
+                else load8_tail(x + row * ldx + k, K - k, v[u]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const int64_t i = base + u * 256;
+        const unsigned s = scale_byte(quad_max(amax8(v[u])));
+        if (i < total) {
+            codes[i] = encode8(v[u], s);
+            if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)s;
+        }
+    }
+}
+
+template <typename T, bool VEC, bool FLAT>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                           int64_t total, int64_t K, int groups, T* __restrict__ out, int64_t ldo) {
+    unsigned c[UNROLL], s[UNROLL];
+    const int64_t base = (int64_t)blockIdx.x * (256 * UNROLL) + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const int64_t i = base + u * 256;
+        c[u] = i < total ? codes[i] : 0u;
+        s[u] = i < total ? scales[i >> 2] : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const int64_t i = base + u * 256;
+        if (i >= total) continue;
+        int64_t row = 0, k = 0;
+        T* p;
+        if constexpr (FLAT) {
+            p = out + i * 8;
+        } else {
+            row = row_of(i, total, groups);
+            k = (i - row * groups) * 8;
+            if (k >= K) continue;
+            p = out + row * ldo + k;
+        }
+        if (FLAT || (VEC && k + 8 <= K)) {
+            if constexpr (sizeof(T) == 4) {
+                float v[8];
+                decode8(c[u], s[u], v);
+                *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            } else if constexpr (__is_same(T, __bf16)) {
+                *reinterpret_cast<bf16x8*>(p) = decode8_bf16(c[u], s[u]);
+            } else {
+                *reinterpret_cast<f16x8*>(p) = decode8_f16(c[u], s[u]);
+            }
+        } else {
+            const int n = K - k < 8 ? (int)(K - k) : 8;
+            T t[8];
+            if constexpr (sizeof(T) == 4) {
+                float v[8];
+                decode8(c[u], s[u], v);
+                for (int j = 0; j < 8; ++j) t[j] = v[j];
+            } else if constexpr (__is_same(T, __bf16)) {
+                const bf16x8 v = decode8_bf16(c[u], s[u]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = v[j];
+            } else {
+                const f16x8 v = decode8_f16(c[u], s[u]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = v[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) p[j] = t[j];
+        }
+    }
+}
+
+template <typename T>
+void quantize_as(const void* xv, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+    const T* x = (const T*)xv;
+    const int64_t groups = code_pitch(K) / 4, total = M * groups;
+    const unsigned grid = (unsigned)ceil_div64(total, 256 * UNROLL);
+    const bool vec = (uintptr_t)x % 16 == 0 && (ldx * sizeof(T)) % 16 == 0;
+    if (vec && K % 128 == 0 && ldx == K)
+        mx_quantize_kernel<T, true, true><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
+    else if (vec)
+        mx_quantize_kernel<T, true, false><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
+    else
+        mx_quantize_kernel<T, false, false><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
+}
+
+template <typename T>
+void dequantize_as(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* ov, int64_t ldo, hipStream_t st) {
+    T* out = (T*)ov;
+    const int64_t groups = code_pitch(K) / 4, total = M * groups;
+    const unsigned grid = (unsigned)ceil_div64(total, 256 * UNROLL);
+    const bool vec = (uintptr_t)out % 16 == 0 && (ldo * sizeof(T)) % 16 == 0;
+    const unsigned* c = (const unsigned*)codes;
+    if (vec && K % 128 == 0 && ldo == K)
+        mx_dequantize_kernel<T, true, true><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
+    else if (vec)
+        mx_dequantize_kernel<T, true, false><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
+    else
+        mx_dequantize_kernel<T, false, false><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
+}
+
+}  // namespace
+
+int launch_quantize(const char* fn, const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
+                    hipStream_t st) {
+    if (dtype == NERF_F32) quantize_as<float>(x, ldx, M, K, codes, scales, st);
+    else if (dtype == NERF_BF16) quantize_as<__bf16>(x, ldx, M, K, codes, scales, st);
+    else quantize_as<_Float16>(x, ldx, M, K, codes, scales, st);
+    return nerf_check_launch(fn);
+}
+
+int launch_dequantize(const char* fn, const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, int dtype, void* out, int64_t ldo,
+                      hipStream_t st) {
+    if (dtype == NERF_F32) dequantize_as<float>(codes, scales, M, K, out, ldo, st);
+    else if (dtype == NERF_BF16) dequantize_as<__bf16>(codes, scales, M, K, out, ldo, st);
+    else dequantize_as<_Float16>(codes, scales, M, K, out, ldo, st);
+    return nerf_check_launch(fn);
+}
+
+}  // namespace mxk
+
+extern "C" size_t nerf_mx_codes_bytes(int64_t rows, int64_t K) {
+    return mxk::sizes_ok(rows, K) ? (size_t)(rows * mxk::code_pitch(K)) : 0;
+}
+extern "C" size_t nerf_mx_scales_bytes(int64_t rows, int64_t K) {
+    return mxk::sizes_ok(rows, K) ? (size_t)(rows * mxk::scale_pitch(K)) : 0;
+}
+
+extern "C" int nerf_mx_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
+                                void* stream) {
+    NERF_REQUIRE(mxk::sizes_ok(M, K) && ldx >= K, "nerf_mx_quantize: bad shape M=%lld K=%lld ldx=%lld", (long long)M, (long long)K,
+                 (long long)ldx);
+    NERF_REQUIRE(dtype >= NERF_F32 && dtype <= NERF_F16, "nerf_mx_quantize: unknown type %d", dtype);
+    if (M == 0) return NERF_OK;
+    NERF_REQUIRE_PTR(x);
+    NERF_REQUIRE_PTR(codes);
+    NERF_REQUIRE_PTR(scales);
+    NERF_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0, "nerf_mx_quantize: codes must be 16-byte, scales 4-byte aligned");
+    return mxk::launch_quantize("nerf_mx_quantize", x, dtype, ldx, M, K, codes, scales, (hipStream_t)stream);
+}
+
+extern "C" int nerf_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, int dtype, void* out, int64_t ldo,
+                                  void* stream) {
+    NERF_REQUIRE(mxk::sizes_ok(M, K) && ldo >= K, "nerf_mx_dequantize: bad shape M=%lld K=%lld ldo=%lld", (long long)M, (long long)K,
+                 (long long)ldo);
+    NERF_REQUIRE(dtype >= NERF_F32 && dtype <= NERF_F16, "nerf_mx_dequantize: unknown type %d", dtype);
+    if (M == 0) return NERF_OK;
+    NERF_REQUIRE_PTR(codes);
+    NERF_REQUIRE_PTR(scales);
+    NERF_REQUIRE_PTR(out);
+    NERF_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0,
+                 "nerf_mx_dequantize: codes must be 16-byte, scales 4-byte aligned");
+    return mxk::launch_dequantize("nerf_mx_dequantize", codes, scales, M, K, dtype, out, ldo, (hipStream_t)stream);
+}

@@ -1,0 +1,810 @@
+// Products of the microscaled 4-bit (MXFP4) operators (format: mx_common.h): one tiled kernel for
+//     forward        y  = post * f(pre * (X W^T + b))     X, W packed     v_mfma_scale_f32_16x16x128_f8f6f4
+//     data gradient  dx = dZ W                            bf16 operands   v_mfma_f32_16x16x32_bf16
+//     weight grad.   dW = dZ^T X                          bf16 operands
+// Both matrix instructions take 64 bytes of a row per step and 16 of them per lane at the same place (row = lane & 15, bytes
+// 16 (lane >> 4) .. +16), and both issue every 16 cycles: staging, LDS image and loop are the same for the two types, only
+// the packed type has scales next to its rows and four times the values per byte.
+//
+// The gradients are those of the product at the rounded operands (straight through the rounding).  X and W as they were
+// rounded are exact in bf16 (a code times a power of two); dz goes in as `terms` bf16 terms (dz = t0 + t1 + t2, each the
+// rounding of what the previous ones left): one for bf16 dy without a smooth activation (exact), two for fp16 dy (11 bits:
+// exact) and for bf16 dy through sin / sigmoid (2^-17, far under the output's own rounding), three for fp32 (exact up to
+// 2^-25).  Sums are fp32 throughout; a split reduction writes fp32 slabs that a second kernel adds in a fixed order.
+#include "mx_common.h"
+#include "sincos.h"
+
+namespace mxk {
+namespace {
+
+enum Kind { PACKED = 0, BF16 = 1 };
+
+struct Operand {
+    const uint8_t* p;       // rows of 64-byte steps
+    int64_t pitch;          // bytes between rows
+    const uint8_t* sc;      // PACKED: four scale bytes per step
+    int64_t sc_pitch;
+    int64_t rows;
+    int64_t plane;          // BF16: bytes between the terms of the operand (0: the same for all terms)
+};
+
+// What happens to a sum on its way out.  slab != NULL: fp32 partial sums [split][M][N], finished by mx_finish_kernel.
+struct Finish {
+    void* out;
+    int64_t ldo;
+    const void* bias;       // type of out, or NULL
+    float pre, post;
+    float* slope;           // sin, sigmoid: d y / d z [M][N] for the gradient, or NULL
+    uint16_t* mask;         // relu: decisions [M][ceil(N / 16)], or NULL
+    float* slab;
+};
+
+struct GemmArgs {
+    Operand w, x;           // out[m][n] = sum over steps of x[m] . w[n]
+    int64_t M;
+    int N;
+    int steps;              // 64-byte steps per row
+    int terms;
+    int per_split;          // stages (two steps) per grid.z slice
+    int tiles_m, tiles_n;
+    Finish f;
+};
+
+template <int ACT>
+__device__ __forceinline__ void activate(float z, const Finish& f, float& y, float& slope) {
+    if constexpr (ACT == NERF_ACT_NONE) {
+        y = f.post * f.pre * z;
+        slope = 0.0f;
+    } else if constexpr (ACT == NERF_ACT_RELU) {
+        const float t = f.pre * z;
+        y = f.post * (t <= 0.0f ? 0.0f : t);   // a NaN stays one
+        slope = t > 0.0f ? 1.0f : 0.0f;
+    } else if constexpr (ACT == NERF_ACT_SIN) {
+        float sn, cs;
+        nerf_sincosf(f.pre * z, &sn, &cs);
+        y = f.post * sn;
+        slope = f.post * f.pre * cs;
+    } else {
+        // exp(-|t|) cannot overflow, and 1 - s would cancel: s and 1 - s are both formed from it
+        const float t = f.pre * z, e = expf(-fabsf(t)), r = 1.0f / (1.0f + e);
+        const float s = t >= 0.0f ? r : e * r;
+        y = f.post * (t != t ? t : s);
+        slope = f.post * f.pre * r * (e * r);
+    }
+}
+
+// four neighbouring outputs of one row (n .. n+3; `count` of them are inside the row)
+template <typename T, int ACT>
+__device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, int n, int N, bool row_ok, const f32x4& bias) {
+    const int count = N - n;
+    f32x4 y, sl;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        activate<ACT>(acc[i] + bias[i], f, a, b);
+        y[i] = a;
+        sl[i] = b;
+    }
+    if constexpr (ACT == NERF_ACT_RELU) {
+        if (f.mask) {   // uniform; the four lanes of a quad hold sixteen neighbours of one row
+            unsigned bits = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bits |= (sl[i] > 0.0f && i < count ? 1u : 0u) << i;
+            bits = quad_or(bits << (4 * (threadIdx.x & 3)));
+            if ((threadIdx.x & 3) == 0 && row_ok && count > 0) f.mask[m * ((N + 15) / 16) + n / 16] = (uint16_t)bits;
+        }
+    }
+    if (!row_ok || count <= 0) return;
+    T* o = (T*)f.out + m * f.ldo + n;
+    typename Vec<T>::x4 t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = (T)y[i];
+    if (count >= 4 && ((uintptr_t)o % sizeof(t)) == 0) {
+        *reinterpret_cast<typename Vec<T>::x4*>(o) = t;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < count) o[i] = t[i];
+    }
+    if constexpr (ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID) {
+        if (f.slope) {
+            float* s = f.slope + m * N + n;
+            if (count >= 4 && ((uintptr_t)s % 16) == 0) {
+                *reinterpret_cast<f32x4*>(s) = sl;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < count) s[i] = sl[i];
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 load_bias(const void* bias, int n, int N) {
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < N) b[i] = (float)((const T*)bias)[n + i];
+    }
+    return b;
+}
+
+__device__ __forceinline__ i32x8 wide(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
+
+// global memory -> LDS, 16 (4) bytes per lane one after the other behind dst; every address lies in [base, base + size).
+// (The size must be a literal for the builtin.)
+__device__ __forceinline__ void load_lds16(const uint8_t* base, int size, uint8_t* dst, int voff, int soff) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, size, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 16, voff, soff, 0, 0);
+}
+__device__ __forceinline__ void load_lds4(const uint8_t* base, int size, uint8_t* dst, int voff, int soff) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, size, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 4, voff, soff, 0, 0);
+}
+
+// Tile of TM rows x TN columns of the output, WM x WN waves, two LDS stages of 128 bytes a row.
+//
+// LDS image of a stage: rows of 128 bytes, the 16-byte piece c of row r at place c ^ (r & 7), so that the fragment reads of
+// eight neighbouring rows (ds_read_b128, the same piece of each) touch all banks once.  The loads go straight to LDS
+// (buffer_load ... lds writes lane after lane, so the permutation is applied to the global address; a row's 128 bytes stay
+// one contiguous request).  W is the A operand: a lane then holds four neighbouring n of one m.
+//
+// Order of a stage's two halves: [read the second half's fragments | multiply the first's], then wait for the next stage's
+// loads, barrier, [request the stage after it, read its first fragments | multiply the second half's].  One barrier a stage;
+// loads have a whole stage to arrive.
+template <int KIND, int TM, int TN, int WM, int WN, typename T, int ACT>
+__global__ __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 1) void mx_gemm_kernel(GemmArgs a) {
+    constexpr int NW = WM * WN, MI = TM / WM / 16, NI = TN / WN / 16, R = TM + TN;
+    constexpr int ROWS = R / NW;            // rows a wave stages: all of one operand
+    constexpr int PIECES = ROWS / 8;        // 1 KiB requests: eight rows each
+    constexpr int SPIECES = ROWS * 2 / 64;  // PACKED: requests of 64 scale words, two per row
+    static_assert(TN % ROWS == 0 && ROWS % 32 == 0, "a wave stages rows of one operand");
+    constexpr int STAGE = R * 128 + (KIND == PACKED ? R * 8 : 0);
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4;
+
+    // Tile of this workgroup.  Workgroups go round the eight XCDs; each XCD gets a contiguous run of tiles, walked in
+    // groups of eight tile rows, so that what shares an L2 shares operand rows.
+    const int tiles = a.tiles_m * a.tiles_n;
+    int t = (int)blockIdx.x;
+    {
+        const int per = tiles / 8, extra = tiles % 8, xcd = t & 7, i = t >> 3;
+        t = xcd * per + (xcd < extra ? xcd : extra) + i;
+    }
+    constexpr int GROUP = 8;
+    const int group = t / (GROUP * a.tiles_n), first = group * GROUP;
+    const int height = a.tiles_m - first < GROUP ? a.tiles_m - first : GROUP;
+    const int in_group = t - group * GROUP * a.tiles_n;
+    const int64_t m0 = (int64_t)(first + in_group % height) * TM;
+    const int n0 = in_group / height * TN;
+
+    // what this wave stages
+    const bool is_w = wave * ROWS < TN;
+    const Operand& op = is_w ? a.w : a.x;
+    const int64_t row0 = is_w ? (int64_t)n0 + wave * ROWS : m0 + (wave * ROWS - TN);
+    const int64_t left = op.rows - row0;
+    const int valid = left > ROWS ? ROWS : left < 1 ? 1 : (int)left;   // rows behind the last one repeat it (never stored)
+    const uint8_t* base = op.p + (left < 1 ? op.rows - 1 : row0) * op.pitch;
+    const int col = (lane & 7) ^ (lane >> 3);
+    int voff[PIECES], svoff[SPIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int row = i * 8 + (lane >> 3);
+        voff[i] = (row < valid ? row : valid - 1) * (int)op.pitch + col * 16;
+    }
+    const uint8_t* sbase = nullptr;
+    if constexpr (KIND == PACKED) {
+        sbase = op.sc + (left < 1 ? op.rows - 1 : row0) * op.sc_pitch;
+#pragma unroll
+        for (int i = 0; i < SPIECES; ++i) {
+            const int row = i * 32 + (lane >> 1);
+            svoff[i] = (row < valid ? row : valid - 1) * (int)op.sc_pitch + (lane & 1) * 4;
+        }
+    }
+    const int stages = (a.steps + 1) / 2;
+    const bool odd = a.steps & 1;
+    const int total = stages * a.terms;
+    const int g0 = (int)blockIdx.z * a.per_split, g1 = g0 + a.per_split < total ? g0 + a.per_split : total;
+
+    int load_term = g0 / stages, load_st = g0 - load_term * stages;   // stage to request next
+    auto request = [&](int buf) {
+        uint8_t* dst = smem + buf * STAGE + wave * (ROWS * 128);
+        // an odd number of steps: the last stage's second half does not exist; it is read from the first (and not used)
+        const bool half = odd && load_st == stages - 1;
+        const int back = half && col >= 4 ? 64 : 0;
+        const uint8_t* from = base + load_term * op.plane;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) load_lds16(from, valid * (int)op.pitch, dst + i * 1024, voff[i] - back, load_st * 128);
+        if constexpr (KIND == PACKED) {
+            uint8_t* sdst = smem + buf * STAGE + R * 128 + wave * (ROWS * 8);
+            const int sback = half && (lane & 1) ? 4 : 0;
+#pragma unroll
+            for (int i = 0; i < SPIECES; ++i)
+                load_lds4(sbase, valid * (int)op.sc_pitch, sdst + i * 256, svoff[i] - sback, load_st * 8);
+        }
+        if (++load_st == stages) { load_st = 0; ++load_term; }
+    };
+
+    const int wm = wave / WN, wn = wave % WN;
+    f32x4 acc[NI][MI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    struct Frags {
+        i32x4 w[NI], x[MI];
+        int sw[NI], sx[MI];
+    } fr[2];
+    const int place[2] = {r * 128 + ((q ^ (r & 7)) * 16), r * 128 + (((4 + q) ^ (r & 7)) * 16)};
+    auto read = [&](Frags& f, int buf, int half) {
+        const uint8_t* wl = smem + buf * STAGE + wn * (NI * 2048) + place[half];
+        const uint8_t* xl = smem + buf * STAGE + TN * 128 + wm * (MI * 2048) + place[half];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) f.w[i] = *reinterpret_cast<const i32x4*>(wl + i * 2048);
+#pragma unroll
+        for (int j = 0; j < MI; ++j) f.x[j] = *reinterpret_cast<const i32x4*>(xl + j * 2048);
+        if constexpr (KIND == PACKED) {
+            const uint8_t* ws = smem + buf * STAGE + R * 128 + wn * (NI * 128) + r * 8 + half * 4 + q;
+            const uint8_t* xs = smem + buf * STAGE + R * 128 + TN * 8 + wm * (MI * 128) + r * 8 + half * 4 + q;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) f.sw[i] = ws[i * 128];
+#pragma unroll
+            for (int j = 0; j < MI; ++j) f.sx[j] = xs[j * 128];
+        }
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+        for (int j = 0; j < MI; ++j)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                if constexpr (KIND == PACKED)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(f.w[i]), wide(f.x[j]), acc[i][j], 4, 4, 0, f.sw[i],
+                                                                                0, f.sx[j]);
+                else
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, f.w[i]),
+                                                                        __builtin_bit_cast(bf16x8, f.x[j]), acc[i][j], 0, 0, 0);
+            }
+    };
+    auto publish = [&] {   // every wave's requests have landed, every wave has read what it needs of the previous stage
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    int st = load_st;   // stage being multiplied, within its term
+    request(0);
+    publish();
+    if (g0 + 1 < g1) request(1);
+    read(fr[0], 0, 0);
+    for (int g = g0; g < g1; ++g) {
+        const int buf = (g - g0) & 1;
+        const bool two = !(odd && st == stages - 1);
+        if (++st == stages) st = 0;
+        if (two) read(fr[1], buf, 1);
+        multiply(fr[0]);
+        if (g + 1 < g1) {
+            publish();
+            if (g + 2 < g1) request(buf);
+            read(fr[0], buf ^ 1, 0);
+        }
+        if (two) multiply(fr[1]);
+    }
+
+    // Out through LDS, two tile rows (32 m) of every wave at a time: the accumulators hold four n of one m per lane, the
+    // stores then take whole rows of the wave's tile.  No request is in flight; the barrier lets the last readers finish.
+    constexpr int WNN = TN / WN, PITCH = WNN + 4;      // floats; 16 bytes of padding spread the rows over the banks
+    constexpr int LPR = WNN / 4, RPI = 64 / LPR;       // lanes per row, rows per instruction
+    static_assert(NW * 32 * PITCH * 4 <= 2 * STAGE, "the way out fits the stages");
+    __syncthreads();
+    float* out_lds = reinterpret_cast<float*>(smem) + wave * (32 * PITCH);
+    const int n = n0 + wn * WNN + (lane % LPR) * 4;
+    const f32x4 bias = a.f.slab ? f32x4{0.f, 0.f, 0.f, 0.f} : load_bias<T>(a.f.bias, n, a.N);
+#pragma unroll
+    for (int jj = 0; jj < MI; jj += 2) {
+#pragma unroll
+        for (int j = jj; j < jj + 2; ++j)
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                *reinterpret_cast<f32x4*>(out_lds + ((j - jj) * 16 + r) * PITCH + i * 16 + q * 4) = acc[i][j];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int row = 0; row < 32; row += RPI) {
+            const int lr = row + lane / LPR;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(out_lds + lr * PITCH + (lane % LPR) * 4);
+            const int64_t m = m0 + wm * (MI * 16) + jj * 16 + lr;
+            if (a.f.slab) {
+                float* s = a.f.slab + ((int64_t)blockIdx.z * a.M + m) * a.N + n;
+                if (m < a.M) {
+                    if (n + 4 <= a.N && a.N % 4 == 0) *reinterpret_cast<f32x4*>(s) = v;
+                    else
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (n + i < a.N) s[i] = v[i];
+                }
+            } else {
+                finish4<T, ACT>(a.f, v, m, n, a.N, m < a.M, bias);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// out = finish(sum of the slabs, in their order)
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void mx_finish_kernel(Finish f, int64_t M, int N, int splits) {
+    const int quads = (N + 15) / 16 * 4;    // groups of four, whole quads of lanes inside a row
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t m = i / quads;
+    const int n = (int)(i - m * quads) * 4;
+    const bool ok = m < M;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (ok && n < N) {
+        const float* s = f.slab + m * N + n;
+        const int64_t step = M * N;
+        if (N % 4 == 0) {
+            for (int z = 0; z < splits; ++z) v += *reinterpret_cast<const f32x4*>(s + z * step);
+        } else {
+            for (int z = 0; z < splits; ++z)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n + j < N) v[j] += s[z * step + j];
+        }
+    }
+    finish4<T, ACT>(f, v, m, n, N, ok, load_bias<T>(f.bias, n, N));
+}
+
+// ---------------------------------------------------------------------------------------------- gradients: operands
+// dz = dy * (d y / d z), split into bf16 terms: rows [term][M][Np] for the data gradient and, turned, [term][N][Mp] for
+// the weight gradient (either may be NULL); Np, Mp: rounded up to 64, zeros behind the end.  colsum: partial column sums
+// of dz [grid.y][N], or NULL.  Tiles of 64 x 64 through LDS, `deep` of them one under the other per workgroup.
+template <int TERMS>
+__device__ __forceinline__ void split_terms(float v, __bf16 (&t)[TERMS]) {
+    const float top = __builtin_bit_cast(float, 0x7f7f0000u);   // largest bf16: fp32 values above it would round to infinity
+    const bool finite = fabsf(v) < __builtin_inff();
+    t[0] = (__bf16)(finite ? fminf(fmaxf(v, -top), top) : v);
+#pragma unroll
+    for (int i = 1; i < TERMS; ++i) {
+        v = finite ? v - (float)t[i - 1] : 0.0f;                // exact
+        t[i] = (__bf16)v;
+    }
+}
+
+struct DzArgs {
+    const void* dy;
+    int64_t lddy;
+    const float* slope;
+    const uint16_t* mask;
+    float factor;
+    int64_t M;
+    int N;
+    int64_t Np, Mp;
+    __bf16* rows;
+    __bf16* turned;
+    float* colsum;
+    int deep;
+};
+
+template <typename T, int TERMS>
+__global__ __launch_bounds__(256) void mx_dz_kernel(DzArgs a) {
+    __shared__ float tile[64 * 65];
+    const int tid = threadIdx.x;
+    const int n0 = blockIdx.x * 64;
+    const int lr = tid >> 2, lc = (tid & 3) * 16;     // reading: a row, sixteen columns
+    float csum = 0.0f;
+    for (int d = 0; d < a.deep; ++d) {
+        const int64_t m0 = ((int64_t)blockIdx.y * a.deep + d) * 64;
+        if (m0 >= a.Mp) break;
+        const int64_t m = m0 + lr;
+        float v[16];
+        const T* p = (const T*)a.dy + m * a.lddy + n0 + lc;
+        const bool in_row = m < a.M;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+        if (in_row) {
+            if (n0 + lc + 16 <= a.N && ((uintptr_t)p % 16) == 0) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 8) {
+                    float t[8];
+                    load8(p + i, t);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i + j] = t[j];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (n0 + lc + i < a.N) v[i] = (float)p[i];
+            }
+            if (a.mask) {
+                unsigned bits = n0 + lc < a.N ? a.mask[m * ((a.N + 15) / 16) + (n0 + lc) / 16] : 0u;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = (bits >> i) & 1u ? v[i] : 0.0f;
+            }
+            if (a.slope) {
+                const float* s = a.slope + m * a.N + n0 + lc;
+                if (n0 + lc + 16 <= a.N && ((uintptr_t)s % 16) == 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const f32x4 t = *reinterpret_cast<const f32x4*>(s + i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[i + j] *= t[j];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (n0 + lc + i < a.N) v[i] *= s[i];
+                }
+            }
+        }
+        if (a.rows && m < a.M) {
+            __bf16 t[16][TERMS];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) split_terms<TERMS>(v[i], t[i]);
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) {
+                __bf16* o = a.rows + ((int64_t)k * a.M + m) * a.Np + n0 + lc;
+                bf16x8 lo, hi;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { lo[i] = t[i][k]; hi[i] = t[8 + i][k]; }
+                *reinterpret_cast<bf16x8*>(o) = lo;
+                *reinterpret_cast<bf16x8*>(o + 8) = hi;
+            }
+        }
+        if (a.turned || a.colsum) {
+            __syncthreads();    // the previous tile has been read
+#pragma unroll
+            for (int i = 0; i < 16; ++i) tile[lr * 65 + lc + i] = v[i];
+            __syncthreads();
+            const int nn = tid >> 2, mm = (tid & 3) * 16;   // writing: a column, sixteen rows
+            __bf16 t[16][TERMS];
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = tile[(mm + i) * 65 + nn];
+                s += x;
+                split_terms<TERMS>(x, t[i]);
+            }
+            csum += s;
+            if (a.turned && n0 + nn < a.N) {
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k) {
+                    __bf16* o = a.turned + ((int64_t)k * a.N + n0 + nn) * a.Mp + m0 + mm;
+                    bf16x8 lo, hi;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { lo[i] = t[i][k]; hi[i] = t[8 + i][k]; }
+                    *reinterpret_cast<bf16x8*>(o) = lo;
+                    *reinterpret_cast<bf16x8*>(o + 8) = hi;
+                }
+            }
+        }
+    }
+    if (a.colsum) {     // the quad's four partial sums, always in the same order
+        csum += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, csum), 0xB1, 0xf, 0xf, true));
+        csum += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, csum), 0x4E, 0xf, 0xf, true));
+        if ((tid & 3) == 0 && n0 + (tid >> 2) < a.N) a.colsum[(int64_t)blockIdx.y * a.N + n0 + (tid >> 2)] = csum * a.factor;
+    }
+}
+
+// db[n] = sum of the partial column sums: a workgroup takes 16 columns, sixteen threads walk each, joined in order
+template <typename T>
+__global__ __launch_bounds__(256) void mx_colsum_kernel(const float* __restrict__ part, int parts, int N, T* __restrict__ db) {
+    __shared__ float s[16][17];
+    const int c = threadIdx.x & 15, w = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
+    float v = 0.0f;
+    if (n < N)
+        for (int i = w; i < parts; i += 16) v += part[(int64_t)i * N + n];
+    s[w][c] = v;
+    __syncthreads();
+    if (w == 0 && n < N) {
+        float sum = 0.0f;
+        for (int i = 0; i < 16; ++i) sum += s[i][c];
+        db[n] = (T)sum;
+    }
+}
+
+// packed rows [rows][K] -> turned bf16 values [K][rows_p], zeros behind the last row.  Tiles of 64 rows x 128 values.
+__global__ __launch_bounds__(256) void mx_turn_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
+                                                     int64_t K, int64_t rows_p, __bf16* __restrict__ out) {
+    __shared__ __bf16 tile[64 * 130];
+    const int tid = threadIdx.x;
+    const int64_t m0 = (int64_t)blockIdx.y * 64, k0 = (int64_t)blockIdx.x * 128;
+    const int64_t m = m0 + (tid >> 2);
+    u32x4 c = {0u, 0u, 0u, 0u};
+    unsigned s = 0;
+    if (m < rows) {
+        const int64_t block = m * scale_pitch(K) + k0 / 32 + (tid & 3);
+        c = *reinterpret_cast<const u32x4*>(codes + block * 16);
+        s = scales[block];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bf16x8 v = decode8_bf16(c[i], s);
+        unsigned* o = reinterpret_cast<unsigned*>(tile + (tid >> 2) * 130 + (tid & 3) * 32 + i * 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = __builtin_bit_cast(unsigned, bf16x2{v[2 * j], v[2 * j + 1]});
+    }
+    __syncthreads();
+    const int kk = tid >> 1, mm = (tid & 1) * 32;
+    if (k0 + kk < K) {
+        __bf16* o = out + (k0 + kk) * rows_p + m0 + mm;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            bf16x8 v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = tile[(mm + i + j) * 130 + kk];
+            *reinterpret_cast<bf16x8*>(o + i) = v;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+constexpr int kTargetGroups = 256;   // compute units
+
+struct Plan {
+    int tiles_m, tiles_n, splits, per_split;
+    size_t slab_floats;
+};
+
+// Tile and split of an M x N product over `total` stages.
+Plan plan_for(int64_t M, int64_t N, int64_t total) {
+    Plan p{};
+    const int t = 128;
+    p.tiles_m = (int)ceil_div64(M, t);
+    p.tiles_n = (int)ceil_div64(N, t);
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    int64_t splits = 1;
+    if (tiles < kTargetGroups) {
+        splits = kTargetGroups / tiles;
+        const int64_t most = total / 4 < 1 ? 1 : total / 4;    // at least four stages a slice
+        if (splits > most) splits = most;
+        if (splits > 256) splits = 256;
+    }
+    p.per_split = (int)ceil_div64(total, splits);
+    p.splits = (int)ceil_div64(total, p.per_split);
+    p.slab_floats = p.splits > 1 ? (size_t)p.splits * M * N : 0;
+    return p;
+}
+
+template <int KIND, int TILE, typename T, int ACT>
+int launch_gemm_tile(const char* fn, const GemmArgs& a, int splits, hipStream_t st) {
+    constexpr int lds = 2 * (2 * TILE * 128 + (KIND == PACKED ? 2 * TILE * 8 : 0));
+    int rc = nerf_set_lds(mx_gemm_kernel<KIND, TILE, TILE, 2, 2, T, ACT>, lds);
+    if (rc) return rc;
+    mx_gemm_kernel<KIND, TILE, TILE, 2, 2, T, ACT><<<dim3((unsigned)(a.tiles_m * a.tiles_n), 1, (unsigned)splits), 256, lds, st>>>(a);
+    return nerf_check_launch(fn);
+}
+
+template <int KIND, typename T, int ACT>
+int launch_gemm(const char* fn, GemmArgs a, const Plan& p, hipStream_t st) {
+    a.tiles_m = p.tiles_m;
+    a.tiles_n = p.tiles_n;
+    a.per_split = p.per_split;
+    if (p.splits == 1) a.f.slab = nullptr;
+    int rc = launch_gemm_tile<KIND, 128, T, ACT>(fn, a, p.splits, st);
+    if (rc || p.splits == 1) return rc;
+    const int64_t items = a.M * ((a.N + 15) / 16 * 4);
+    mx_finish_kernel<T, ACT><<<(unsigned)ceil_div64(items, 256), 256, 0, st>>>(a.f, a.M, a.N, p.splits);
+    return nerf_check_launch(fn);
+}
+
+template <typename T>
+int launch_forward(const char* fn, const GemmArgs& a, const Plan& p, int act, hipStream_t st) {
+    if (act == NERF_ACT_NONE) return launch_gemm<PACKED, T, NERF_ACT_NONE>(fn, a, p, st);
+    if (act == NERF_ACT_RELU) return launch_gemm<PACKED, T, NERF_ACT_RELU>(fn, a, p, st);
+    if (act == NERF_ACT_SIN) return launch_gemm<PACKED, T, NERF_ACT_SIN>(fn, a, p, st);
+    return launch_gemm<PACKED, T, NERF_ACT_SIGMOID>(fn, a, p, st);
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+int terms_for(int dtype, int act) {
+    if (dtype == NERF_F32) return 3;
+    if (dtype == NERF_F16) return 2;
+    return act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID ? 2 : 1;
+}
+
+struct FwdLayout {
+    Plan plan;
+    size_t codes, scales, slab, bytes;   // offsets; the quantised x where the caller keeps none
+};
+FwdLayout fwd_layout(int64_t M, int64_t K, int64_t N) {
+    FwdLayout l{};
+    l.plan = plan_for(M, N, ceil_div64(ceil_div64(K, 128), 2));
+    l.codes = 0;
+    l.scales = up256((size_t)(M * code_pitch(K)));
+    l.slab = l.scales + up256((size_t)(M * scale_pitch(K)));
+    l.bytes = l.slab + l.plan.slab_floats * 4;
+    return l;
+}
+
+struct BwdLayout {
+    int terms, deep;
+    int64_t Np, Mp, parts;
+    Plan dx, dw;
+    size_t rows, turned, part, wt, xt, slab, bytes;
+};
+BwdLayout bwd_layout(int dtype, int act, int64_t M, int64_t K, int64_t N, bool need_dx, bool need_dw, bool need_db) {
+    BwdLayout l{};
+    l.terms = terms_for(dtype, act);
+    l.Np = ceil_div64(N, 64) * 64;
+    l.Mp = ceil_div64(M, 64) * 64;
+    const int64_t tiles = (l.Np / 64) * (l.Mp / 64);
+    l.deep = tiles >= 8192 ? 8 : tiles >= 2048 ? 2 : 1;
+    l.parts = ceil_div64(l.Mp / 64, l.deep);
+    l.dx = plan_for(M, K, l.Np / 64 * l.terms);
+    l.dw = plan_for(N, K, l.Mp / 64 * l.terms);
+    size_t at = 0;
+    l.rows = at;
+    if (need_dx) at += up256((size_t)l.terms * M * l.Np * 2);
+    l.turned = at;
+    if (need_dw) at += up256((size_t)l.terms * N * l.Mp * 2);
+    l.part = at;
+    if (need_db) at += up256((size_t)l.parts * N * 4);
+    l.wt = at;
+    if (need_dx) at += up256((size_t)K * l.Np * 2);
+    l.xt = at;
+    if (need_dw) at += up256((size_t)K * l.Mp * 2);
+    l.slab = at;
+    const size_t s1 = need_dx ? l.dx.slab_floats : 0, s2 = need_dw ? l.dw.slab_floats : 0;
+    at += (s1 > s2 ? s1 : s2) * 4;   // one after the other on one stream
+    l.bytes = at;
+    return l;
+}
+
+template <typename T>
+int launch_dz(const char* fn, const DzArgs& a, int terms, hipStream_t st) {
+    const dim3 grid((unsigned)(a.Np / 64), (unsigned)ceil_div64(a.Mp / 64, a.deep));
+    if (terms == 1) mx_dz_kernel<T, 1><<<grid, 256, 0, st>>>(a);
+    else if (terms == 2) mx_dz_kernel<T, 2><<<grid, 256, 0, st>>>(a);
+    else mx_dz_kernel<T, 3><<<grid, 256, 0, st>>>(a);
+    return nerf_check_launch(fn);
+}
+
+template <typename T>
+int backward(const char* fn, const BwdLayout& l, DzArgs dz, const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes,
+             const uint8_t* wscales, int64_t M, int64_t K, int64_t N, uint8_t* ws, void* dx, int64_t lddx, void* dw, void* db,
+             hipStream_t st) {
+    dz.rows = dx ? (__bf16*)(ws + l.rows) : nullptr;
+    dz.turned = dw ? (__bf16*)(ws + l.turned) : nullptr;
+    dz.colsum = db ? (float*)(ws + l.part) : nullptr;
+    int rc = launch_dz<T>(fn, dz, l.terms, st);
+    if (rc) return rc;
+    if (db) {
+        mx_colsum_kernel<T><<<(unsigned)ceil_div64(N, 16), 256, 0, st>>>(dz.colsum, (int)l.parts, (int)N, (T*)db);
+        if ((rc = nerf_check_launch(fn))) return rc;
+    }
+    if (dx) {   // dx[m][k] = sum over n of dz[m][n] W[n][k]
+        mx_turn_kernel<<<dim3((unsigned)ceil_div64(K, 128), (unsigned)(l.Np / 64)), 256, 0, st>>>(wcodes, wscales, N, K, l.Np,
+                                                                                                 (__bf16*)(ws + l.wt));
+        if ((rc = nerf_check_launch(fn))) return rc;
+        GemmArgs a{};
+        a.w = Operand{ws + l.wt, l.Np * 2, nullptr, 0, K, 0};
+        a.x = Operand{ws + l.rows, l.Np * 2, nullptr, 0, M, M * l.Np * 2};
+        a.M = M;
+        a.N = (int)K;
+        a.steps = (int)(l.Np / 32);
+        a.terms = l.terms;
+        a.f = Finish{dx, lddx, nullptr, 1.0f, dz.factor, nullptr, nullptr, (float*)(ws + l.slab)};
+        if ((rc = launch_gemm<BF16, T, NERF_ACT_NONE>(fn, a, l.dx, st))) return rc;
+    }
+    if (dw) {   // dW[n][k] = sum over m of dz[m][n] X[m][k]
+        mx_turn_kernel<<<dim3((unsigned)ceil_div64(K, 128), (unsigned)(l.Mp / 64)), 256, 0, st>>>(xcodes, xscales, M, K, l.Mp,
+                                                                                                 (__bf16*)(ws + l.xt));
+        if ((rc = nerf_check_launch(fn))) return rc;
+        GemmArgs a{};
+        a.w = Operand{ws + l.xt, l.Mp * 2, nullptr, 0, K, 0};
+        a.x = Operand{ws + l.turned, l.Mp * 2, nullptr, 0, N, N * l.Mp * 2};
+        a.M = N;
+        a.N = (int)K;
+        a.steps = (int)(l.Mp / 32);
+        a.terms = l.terms;
+        a.f = Finish{dw, K, nullptr, 1.0f, dz.factor, nullptr, nullptr, (float*)(ws + l.slab)};
+        if ((rc = launch_gemm<BF16, T, NERF_ACT_NONE>(fn, a, l.dw, st))) return rc;
+    }
+    return NERF_OK;
+}
+
+}  // namespace
+}  // namespace mxk
+
+using namespace mxk;
+
+// M up to 2^30 rows, K and N up to 2^22: 32-bit offsets inside a tile, int tile counts
+static bool linear_sizes_ok(int64_t M, int64_t K, int64_t N) {
+    return M >= 0 && M <= (1 << 30) && K >= 1 && K <= (1 << 22) && N >= 1 && N <= (1 << 22) &&
+           ceil_div64(M, 128) * ceil_div64(N, 128) <= (1 << 30);
+}
+
+extern "C" size_t nerf_mx_linear_fwd_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+    return linear_sizes_ok(M, K, N) && M > 0 ? fwd_layout(M, K, N).bytes : 0;
+}
+
+extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales, const void* bias,
+                                  int64_t M, int64_t K, int64_t N, int act, double pre, double post, void* y, int64_t ldy, float* slope,
+                                  uint16_t* mask, uint8_t* xcodes, uint8_t* xscales, void* workspace, void* stream) {
+    const char* fn = "nerf_mx_linear_fwd";
+    NERF_REQUIRE(linear_sizes_ok(M, K, N) && ldx >= K && ldy >= N, "%s: bad shape M=%lld K=%lld N=%lld ldx=%lld ldy=%lld", fn, (long long)M,
+                 (long long)K, (long long)N, (long long)ldx, (long long)ldy);
+    NERF_REQUIRE(dtype >= NERF_F32 && dtype <= NERF_F16, "%s: unknown type %d", fn, dtype);
+    NERF_REQUIRE(act >= NERF_ACT_NONE && act <= NERF_ACT_SIGMOID, "%s: unknown activation %d", fn, act);
+    if (M == 0) return NERF_OK;
+    NERF_REQUIRE_PTR(x);
+    NERF_REQUIRE_PTR(wcodes);
+    NERF_REQUIRE_PTR(wscales);
+    NERF_REQUIRE_PTR(y);
+    NERF_REQUIRE_PTR(workspace);
+    NERF_REQUIRE((xcodes == nullptr) == (xscales == nullptr), "%s: xcodes and xscales go together", fn);
+    NERF_REQUIRE((uintptr_t)wcodes % 16 == 0 && (uintptr_t)wscales % 4 == 0 && (uintptr_t)xcodes % 16 == 0 && (uintptr_t)xscales % 4 == 0 &&
+                     (uintptr_t)workspace % 16 == 0,
+                 "%s: codes and workspace must be 16-byte, scales 4-byte aligned", fn);
+    const hipStream_t st = (hipStream_t)stream;
+    const FwdLayout l = fwd_layout(M, K, N);
+    uint8_t* ws = (uint8_t*)workspace;
+    uint8_t* xc = xcodes ? xcodes : ws + l.codes;
+    uint8_t* xs = xscales ? xscales : ws + l.scales;
+    int rc = launch_quantize(fn, x, dtype, ldx, M, K, xc, xs, st);
+    if (rc) return rc;
+    GemmArgs a{};
+    a.w = Operand{wcodes, code_pitch(K), wscales, scale_pitch(K), N, 0};
+    a.x = Operand{xc, code_pitch(K), xs, scale_pitch(K), M, 0};
+    a.M = M;
+    a.N = (int)N;
+    a.steps = (int)ceil_div64(K, 128);
+    a.terms = 1;
+    a.f = Finish{y, ldy, bias, (float)pre, (float)post, act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID ? slope : nullptr,
+                 act == NERF_ACT_RELU ? mask : nullptr, (float*)(ws + l.slab)};
+    if (dtype == NERF_F32) return launch_forward<float>(fn, a, l.plan, act, st);
+    if (dtype == NERF_BF16) return launch_forward<__bf16>(fn, a, l.plan, act, st);
+    return launch_forward<_Float16>(fn, a, l.plan, act, st);
+}
+
+extern "C" size_t nerf_mx_linear_bwd_workspace_bytes(int dtype, int act, int64_t M, int64_t K, int64_t N, int need_dx, int need_dw,
+                                                     int need_db) {
+    if (!linear_sizes_ok(M, K, N) || M < 1 || dtype < NERF_F32 || dtype > NERF_F16) return 0;
+    return bwd_layout(dtype, act, M, K, N, need_dx, need_dw, need_db).bytes;
+}
+
+extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const float* slope, const uint16_t* mask, int act, double pre,
+                                  double post, const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes,
+                                  const uint8_t* wscales, int64_t M, int64_t K, int64_t N, void* workspace, void* dx, int64_t lddx,
+                                  void* dw, void* db, void* stream) {
+    const char* fn = "nerf_mx_linear_bwd";
+    NERF_REQUIRE(linear_sizes_ok(M, K, N) && M >= 1 && lddy >= N && (!dx || lddx >= K), "%s: bad shape M=%lld K=%lld N=%lld", fn,
+                 (long long)M, (long long)K, (long long)N);
+    NERF_REQUIRE(dtype >= NERF_F32 && dtype <= NERF_F16, "%s: unknown type %d", fn, dtype);
+    NERF_REQUIRE(act >= NERF_ACT_NONE && act <= NERF_ACT_SIGMOID, "%s: unknown activation %d", fn, act);
+    NERF_REQUIRE(M <= 65535ll * 64, "%s: more than 65535*64 rows per call", fn);   // grid.y; 32-bit offsets inside a turned tile
+    if (!dx && !dw && !db) return NERF_OK;
+    NERF_REQUIRE_PTR(dy);
+    NERF_REQUIRE_PTR(workspace);
+    if (act == NERF_ACT_RELU) NERF_REQUIRE_PTR(mask);
+    if (act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID) NERF_REQUIRE_PTR(slope);
+    if (dx) { NERF_REQUIRE_PTR(wcodes); NERF_REQUIRE_PTR(wscales); }
+    if (dw) { NERF_REQUIRE_PTR(xcodes); NERF_REQUIRE_PTR(xscales); }
+    NERF_REQUIRE((uintptr_t)wcodes % 16 == 0 && (uintptr_t)xcodes % 16 == 0 && (uintptr_t)workspace % 16 == 0,
+                 "%s: codes and workspace must be 16-byte aligned", fn);
+    const BwdLayout l = bwd_layout(dtype, act, M, K, N, dx != nullptr, dw != nullptr, db != nullptr);
+    DzArgs dz{};
+    dz.dy = dy;
+    dz.lddy = lddy;
+    dz.slope = act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID ? slope : nullptr;
+    dz.mask = act == NERF_ACT_RELU ? mask : nullptr;
+    // the constant factor of dz stays out of the terms (they are exact without it) and is applied to the sums
+    dz.factor = dz.slope ? 1.0f : (float)(pre * post);
+    dz.M = M;
+    dz.N = (int)N;
+    dz.Np = l.Np;
+    dz.Mp = l.Mp;
+    dz.deep = l.deep;
+    const hipStream_t st = (hipStream_t)stream;
+    uint8_t* ws = (uint8_t*)workspace;
+    if (dtype == NERF_F32)
+        return backward<float>(fn, l, dz, xcodes, xscales, wcodes, wscales, M, K, N, ws, dx, lddx, dw, db, st);
+    if (dtype == NERF_BF16)
+        return backward<__bf16>(fn, l, dz, xcodes, xscales, wcodes, wscales, M, K, N, ws, dx, lddx, dw, db, st);
+    return backward<_Float16>(fn, l, dz, xcodes, xscales, wcodes, wscales, M, K, N, ws, dx, lddx, dw, db, st);
+}

@@ -4,7 +4,8 @@ Poses as reference eval.py:14-41,91-97 (theta sweep, phi = -30 deg, radius 4), r
 on the device, frames quantised as (clip(rgb,0,1)*255) truncated to uint8 (eval.py:149-150) and
 written as PNG.  With torchrun the poses are sharded over ranks (no collective).  A checkpoint of a
 coarse + fine pair (train.py with `num_fine_samples`) is rendered hierarchically; `--precision bf16`
-or `bf16x3` selects the opt-in inference kernels on the bf16 matrix pipe (NeRF only; bf16x3 keeps fp32 accuracy)."""
+or `bf16x3` selects the opt-in inference kernels on the bf16 matrix pipe (NeRF only; bf16x3 keeps fp32 accuracy);
+`--precision mxfp4` renders the microscaled 4-bit network (train.py `train_precision = mxfp4`; single networks only)."""
 import argparse
 import os
 import sys
@@ -66,7 +67,7 @@ def main(argv=None):
     ap.add_argument('--checkpoint', type=str, required=True)
     ap.add_argument('--output', type=str, default='rendered_frames')
     ap.add_argument('--resolution', type=int, default=None, help='override H=W (default: the test image size)')
-    ap.add_argument('--precision', choices=['fp32', 'bf16', 'bf16x3'], default='fp32')
+    ap.add_argument('--precision', choices=['fp32', 'bf16', 'bf16x3', 'mxfp4'], default='fp32')
     ap.add_argument('--one-device', action='store_true', help='rehearsal only: every rank renders on cuda:0')
     args = ap.parse_args(argv)
     cfg = parse_config(args.config)
@@ -89,6 +90,8 @@ def main(argv=None):
     make = NeRF if model_type == 'nerf' else Siren
     state = ckpt['model_state_dict']
     pair = any(k.startswith('coarse.') for k in state)
+    if pair and args.precision == 'mxfp4':
+        raise ValueError("--precision mxfp4 renders single networks; this checkpoint holds a coarse + fine pair")
     if pair:
         model = torch.nn.ModuleDict({"coarse": make(), "fine": make()}).to(device)
         nets = [model["coarse"], model["fine"]]

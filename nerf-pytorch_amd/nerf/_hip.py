@@ -72,6 +72,16 @@ _SIGS = {
     "nerf_weights_to_cdf": (c_int, [_P, c_int64, c_int, _P, _P]),
     "nerf_sample_pdf": (c_int, [_P, _P, _P, c_int64, c_int, c_int, _P, _P, _P]),
     "nerf_resample": (c_int, [_P, _P, _P, c_int64, c_int, c_int, _P, _P, _P, _P, _P]),
+    "nerf_mx_codes_bytes": (c_size_t, [c_int64, c_int64]),
+    "nerf_mx_scales_bytes": (c_size_t, [c_int64, c_int64]),
+    "nerf_mx_quantize": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, _P, _P]),
+    "nerf_mx_dequantize": (c_int, [_P, _P, c_int64, c_int64, c_int, _P, c_int64, _P]),
+    "nerf_mx_linear_fwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "nerf_mx_linear_fwd": (c_int, [_P, c_int, c_int64, _P, _P, _P, c_int64, c_int64, c_int64, c_int, c_double, c_double, _P, c_int64,
+                                   _P, _P, _P, _P, _P, _P]),
+    "nerf_mx_linear_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_int]),
+    "nerf_mx_linear_bwd": (c_int, [_P, c_int, c_int64, _P, _P, c_int, c_double, c_double, _P, _P, _P, _P, c_int64, c_int64, c_int64,
+                                   _P, _P, c_int64, _P, _P, _P]),
 }
 EXPORTS = tuple(_SIGS)
 for _name, (_res, _args) in _SIGS.items():
@@ -486,3 +496,128 @@ def resample(weights: torch.Tensor, t_coarse: torch.Tensor, u: torch.Tensor, wan
                              _dev(deltas, "deltas"), _opt(t_fine, "t_fine"),
                              None if idx is None else _dev(idx, "idx", torch.int32), _stream()), "nerf_resample")
     return (t_all, deltas, t_fine, idx) if want_fine else (t_all, deltas)
+
+
+# --------------------------------------------------------------------------- microscaled 4-bit rows (nerf/mx.py)
+MX_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _mx_dtype(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in MX_DTYPES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return MX_DTYPES[t.dtype]
+
+
+def _mx_rows(t: torch.Tensor, name: str):
+    """(pointer, row pitch in elements) of a matrix whose rows may lie apart but are contiguous themselves."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: tensor is on {t.device}; this build runs on a HIP device only (no CPU path)")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{name}: expected a matrix with contiguous rows that do not overlap")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _mx_stream(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _on_device(t: torch.Tensor):
+    """The launches go to the current device: make it the tensor's."""
+    return torch.cuda.device(t.device)
+
+
+def mx_packed_shape(rows: int, K: int):
+    """Shapes of the codes and scales of `rows` packed rows of K values."""
+    blocks = (K + 127) // 128
+    return (rows, 64 * blocks), (rows, 4 * blocks)
+
+
+def _mx_packed(codes: torch.Tensor, scales: torch.Tensor, K: int, name: str):
+    c, s = mx_packed_shape(codes.shape[0], K)
+    if tuple(codes.shape) != c or tuple(scales.shape) != s:
+        raise ValueError(f"{name}: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} are not packed rows of {K} values")
+    if codes.device != scales.device:
+        raise ValueError(f"{name}: codes and scales are on different devices")
+    return _dev(codes, f"{name}.codes", torch.uint8), _dev(scales, f"{name}.scales", torch.uint8)
+
+
+def _mx_alloc(rows: int, K: int, device):
+    c, s = mx_packed_shape(rows, K)
+    return torch.empty(c, dtype=torch.uint8, device=device), torch.empty(s, dtype=torch.uint8, device=device)
+
+
+def mx_quantize(x: torch.Tensor):
+    """x [M,K] -> (codes, scales)."""
+    dt = _mx_dtype(x, "x")
+    ptr, ld = _mx_rows(x, "x")
+    M, K = x.shape
+    with _on_device(x):
+        codes, scales = _mx_alloc(M, K, x.device)
+        _check(lib.nerf_mx_quantize(ptr, dt, ld, M, K, codes.data_ptr(), scales.data_ptr(), _mx_stream(x)), "nerf_mx_quantize")
+    return codes, scales
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int, dtype) -> torch.Tensor:
+    pc, ps = _mx_packed(codes, scales, K, "packed")
+    if dtype not in MX_DTYPES:
+        raise TypeError(f"expected float32, bfloat16 or float16, got {dtype}")
+    M = codes.shape[0]
+    with _on_device(codes):
+        out = torch.empty((M, K), dtype=dtype, device=codes.device)
+        _check(lib.nerf_mx_dequantize(pc, ps, M, K, MX_DTYPES[dtype], out.data_ptr(), K, _mx_stream(codes)), "nerf_mx_dequantize")
+    return out
+
+
+def mx_linear_fwd(x: torch.Tensor, wcodes: torch.Tensor, wscales: torch.Tensor, b: Optional[torch.Tensor], act: int, pre: float,
+                  post: float, train: bool = False):
+    """y [M,N] = post * f(pre * (Q(x) W^T + b)); with `train` also what the backward needs: (y, slope, mask, xcodes, xscales)."""
+    dt = _mx_dtype(x, "x")
+    ptr, ld = _mx_rows(x, "x")
+    M, K = x.shape
+    N = wcodes.shape[0]
+    pc, ps = _mx_packed(wcodes, wscales, K, "weight")
+    if wcodes.device != x.device or (b is not None and b.device != x.device):
+        raise ValueError("mx_linear: x, weight and bias must be on one device")
+    if b is not None and (b.shape != (N,) or b.dtype != x.dtype):
+        raise ValueError(f"mx_linear: bias must be {x.dtype} [{N}], got {b.dtype} {tuple(b.shape)}")
+    slope = mask = xc = xs = None
+    with _on_device(x):
+        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        if train:
+            if act in (ACT_SIN, ACT_SIGMOID):
+                slope = torch.empty((M, N), dtype=torch.float32, device=x.device)
+            elif act == ACT_RELU:
+                mask = torch.empty((M, (N + 15) // 16), dtype=torch.int16, device=x.device)
+            xc, xs = _mx_alloc(M, K, x.device)
+        ws = torch.empty(lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N), dtype=torch.uint8, device=x.device)
+        ev = timers.start("mx_linear_fwd", M)
+        _check(lib.nerf_mx_linear_fwd(ptr, dt, ld, pc, ps, None if b is None else _dev(b, "b", x.dtype), M, K, N, act, float(pre),
+                                      float(post), y.data_ptr(), N, *(None if t is None else t.data_ptr() for t in (slope, mask, xc, xs)),
+                                      ws.data_ptr(), _mx_stream(x)), "nerf_mx_linear_fwd")
+        timers.stop(ev)
+    return (y, slope, mask, xc, xs) if train else y
+
+
+def mx_linear_bwd(dy: torch.Tensor, slope, mask, act: int, pre: float, post: float, xcodes, xscales, wcodes, wscales, K: int,
+                  need_dx: bool, need_dw: bool, need_db: bool):
+    """(dx [M,K], dW [N,K], db [N]) in the type of dy, None where not asked for."""
+    dt = _mx_dtype(dy, "dy")
+    ptr, ld = _mx_rows(dy, "dy")
+    M, N = dy.shape
+    xp = _mx_packed(xcodes, xscales, K, "x")
+    wp = _mx_packed(wcodes, wscales, K, "weight")
+    if xcodes.shape[0] != M or wcodes.shape[0] != N:
+        raise ValueError(f"mx_linear_bwd: dy {tuple(dy.shape)} does not match x [{xcodes.shape[0]},{K}] and W [{wcodes.shape[0]},{K}]")
+    dev = dy.device
+    with _on_device(dy):
+        dx = torch.empty((M, K), dtype=dy.dtype, device=dev) if need_dx else None
+        dw = torch.empty((N, K), dtype=dy.dtype, device=dev) if need_dw else None
+        db = torch.empty((N,), dtype=dy.dtype, device=dev) if need_db else None
+        ws = torch.empty(lib.nerf_mx_linear_bwd_workspace_bytes(dt, act, M, K, N, need_dx, need_dw, need_db), dtype=torch.uint8, device=dev)
+        ev = timers.start("mx_linear_bwd", M)
+        _check(lib.nerf_mx_linear_bwd(ptr, dt, ld, None if slope is None else slope.data_ptr(), None if mask is None else mask.data_ptr(),
+                                      act, float(pre), float(post), *xp, *wp, M, K, N, ws.data_ptr(),
+                                      None if dx is None else dx.data_ptr(), K, None if dw is None else dw.data_ptr(),
+                                      None if db is None else db.data_ptr(), _mx_stream(dy)), "nerf_mx_linear_bwd")
+        timers.stop(ev)
+    return dx, dw, db

@@ -15,13 +15,16 @@ from typing import List, Tuple
 import torch
 import torch.nn as nn
 
-from . import _hip
+from . import _hip, mx
 from .ops import LinearActFunction, MLPFunction, PackedWeights, _f32c, grad_sink, wants_grad
 
 
 def _dense(x: torch.Tensor, lin: nn.Linear, act: int = _hip.ACT_NONE, pre: float = 1.0, post: float = 1.0,
-           rows: slice = slice(None)) -> torch.Tensor:
-    """post*f(pre*(x W^T + b)) on the layer-wise kernels; `rows` selects output rows of the layer."""
+           rows: slice = slice(None), mxfp4: bool = False) -> torch.Tensor:
+    """post*f(pre*(x W^T + b)) on the layer-wise kernels; `rows` selects output rows of the layer.  mxfp4: on the 4-bit
+    matrix pipe, input and weight rounded on the call."""
+    if mxfp4:
+        return mx.linear(x, lin.weight[rows], lin.bias[rows], act, pre, post)
     return LinearActFunction.apply(x, lin.weight[rows], lin.bias[rows], act, pre, post)
 
 
@@ -51,9 +54,14 @@ class _FusedMLP(nn.Module):
         every product formed from six term products accumulated in fp32 -- fp32 accuracy (the mode holds the fp32
         path's 1e-5 bar, gradients included) at a fraction of the matrix-pipe time; so do the wide weight-gradient
         products (the narrow ones stay on fp32 MFMA).  Both models, default architecture.  Passes without gradients are
-        not affected (see set_inference_precision)."""
-        if precision not in ("fp32", "bf16x3"):
-            raise ValueError("training precision must be 'fp32' or 'bf16x3'")
+        not affected (see set_inference_precision).
+
+        'mxfp4' (any constructor arguments): the layers between hidden activations run on the 4-bit matrix pipe, layer by
+        layer, with inputs and weights rounded to microscaled 4-bit blocks on every pass and gradients straight through
+        the rounding (nerf/mx.py) -- training FOR a 4-bit network, not an approximation of the fp32 one.  Layers that read
+        coordinates or encodings and the output heads stay fp32."""
+        if precision not in ("fp32", "bf16x3", "mxfp4"):
+            raise ValueError("training precision must be 'fp32', 'bf16x3' or 'mxfp4'")
         if precision == "bf16x3":
             self._check_supported()
             if _hip.lib.nerf_mlp_packed_x3_floats(self.model_id) == 0:
@@ -69,10 +77,13 @@ class _FusedMLP(nn.Module):
         encodings and activations are rounded to bf16 and accumulated in fp32 (tolerance of its own).
         'bf16x3': every fp32 operand is split into three bf16 terms and a product is formed from six term
         products accumulated in fp32 -- fp32 accuracy (it holds the fp32 path's parity bar) at about 1.7 times
-        the fp32 kernel's rate; both models.  'bf16' covers NeRF only.  Training always runs fp32."""
-        if precision not in ("fp32", "bf16", "bf16x3"):
-            raise ValueError("precision must be 'fp32', 'bf16' or 'bf16x3'")
-        if precision != "fp32":
+        the fp32 kernel's rate; both models.  'bf16' covers NeRF only.  Training always runs fp32.
+
+        'mxfp4' (any constructor arguments): the network that set_training_precision('mxfp4') trains -- layers between
+        hidden activations on the 4-bit matrix pipe, layer by layer, everything else fp32."""
+        if precision not in ("fp32", "bf16", "bf16x3", "mxfp4"):
+            raise ValueError("precision must be 'fp32', 'bf16', 'bf16x3' or 'mxfp4'")
+        if precision not in ("fp32", "mxfp4"):
             self._check_supported()
             if getattr(_hip.lib, f"nerf_mlp_packed_{precision}_bytes")(self.model_id) == 0:
                 raise NotImplementedError(f"the {precision} inference mode covers the NeRF model only")
@@ -91,7 +102,7 @@ class _FusedMLP(nn.Module):
     def packed_weights(self, train: bool = True) -> torch.Tensor:
         """Weight image for the kernels: the fp32 image, or the bf16 / bf16x3 one for a gradient-free pass of
         a module switched to that inference mode."""
-        if not train and self.inference_precision != "fp32":
+        if not train and self.inference_precision in ("bf16", "bf16x3"):
             return self._packed_bf16.get(self.ordered_parameters())
         return self._packed.get(self.ordered_parameters())
 
@@ -100,6 +111,11 @@ class _FusedMLP(nn.Module):
         self._packed.invalidate()
         if self._packed_bf16 is not None:
             self._packed_bf16.invalidate()
+
+    def runs_mxfp4(self) -> bool:
+        """True when a pass made now runs layer by layer on the 4-bit matrix pipe (no fused kernel, no weight image)."""
+        train = torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())
+        return (self.training_precision if train else self.inference_precision) == "mxfp4"
 
     def fused_supported(self) -> bool:
         """True when the constructor arguments are the ones the fused kernels are built for."""
@@ -119,7 +135,7 @@ class _FusedMLP(nn.Module):
         if points.dim() != 2 or points.shape[1] != 3 or rays_d.shape != points.shape:
             raise ValueError("points and rays_d must both be [M,3]")
         inputs_need_grad = torch.is_grad_enabled() and (points.requires_grad or rays_d.requires_grad)
-        if inputs_need_grad or not self.fused_supported():
+        if inputs_need_grad or not self.fused_supported() or self.runs_mxfp4():
             # The fused kernels produce parameter gradients only (the reference's callers never ask for more).
             # Gradients with respect to points / directions, which the reference's forward also supports, come
             # from the layer-wise kernels: every dense layer and the encoding have an input gradient there.
@@ -151,18 +167,20 @@ class NeRF(_FusedMLP):
 
     def _layerwise(self, points, rays_d):
         """nerf/models.py:62-75 layer by layer; the 257-row last trunk layer is evaluated as its 256
-        feature rows (no activation) and its density row (ReLU) so that no arithmetic is left to ATen."""
+        feature rows (no activation) and its density row (ReLU) so that no arithmetic is left to ATen.  In the mxfp4
+        mode the layers whose whole input are hidden activations take the 4-bit product."""
         from .encoding import positional_encoding
+        fp4 = self.runs_mxfp4()
         pe = positional_encoding(points, self.pos_encoding_dim)
         de = positional_encoding(rays_d, self.dir_encoding_dim)
         h = pe
-        for lin in self.block1[0::2]:
-            h = _dense(h, lin, _hip.ACT_RELU)
+        for i, lin in enumerate(self.block1[0::2]):
+            h = _dense(h, lin, _hip.ACT_RELU, mxfp4=fp4 and i > 0)
         h = torch.cat([h, pe], dim=1)
         trunk = list(self.block2[0::2])
-        for lin in trunk[:-1]:
-            h = _dense(h, lin, _hip.ACT_RELU)
-        feat = _dense(h, trunk[-1], _hip.ACT_NONE, rows=slice(0, self.hidden_dim))
+        for i, lin in enumerate(trunk[:-1]):
+            h = _dense(h, lin, _hip.ACT_RELU, mxfp4=fp4 and i > 0)
+        feat = _dense(h, trunk[-1], _hip.ACT_NONE, rows=slice(0, self.hidden_dim), mxfp4=fp4)
         density = _dense(h, trunk[-1], _hip.ACT_RELU, rows=slice(self.hidden_dim, self.hidden_dim + 1)).squeeze(-1)
         g = _dense(torch.cat([feat, de], dim=1), self.rgb_head[0], _hip.ACT_RELU)
         return _dense(g, self.rgb_head[2], _hip.ACT_SIGMOID), density
@@ -227,13 +245,15 @@ class Siren(_FusedMLP):
 
     def _layerwise(self, points, rays_d):
         """nerf/models.py:185-203 layer by layer (sin(w0 z), relu*sigma_mul and sigmoid(rgb_mul z) are
-        epilogues of the dense kernel)."""
+        epilogues of the dense kernel).  In the mxfp4 mode the layers whose whole input are hidden activations take the
+        4-bit product."""
         from .encoding import positional_encoding
+        fp4 = self.runs_mxfp4()
         h = points
-        for layer in self.block1:
-            h = _dense(h, layer.layer, _hip.ACT_SIN, pre=layer.w0)
+        for i, layer in enumerate(self.block1):
+            h = _dense(h, layer.layer, _hip.ACT_SIN, pre=layer.w0, mxfp4=fp4 and i > 0)
         density = _dense(h, self.density_branch[0], _hip.ACT_RELU, post=self.sigma_mul).squeeze(-1)
-        feat = _dense(h, self.feature_remap[0])
+        feat = _dense(h, self.feature_remap[0], mxfp4=fp4)
         de = positional_encoding(rays_d, self.dir_encoding_dim)
         head = self.rgb_head[0]
         g = _dense(torch.cat([feat, de], dim=1), head.layer, _hip.ACT_SIN, pre=head.w0)

@@ -314,6 +314,35 @@ class LinearActFunction(torch.autograd.Function):
         return dx, dW, db, None, None, None
 
 
+class MXLinearFunction(torch.autograd.Function):
+    """y = post * f(pre * (Q(x) Q(W)^T + b)) on the 4-bit matrix pipe (nerf/mx.py).  The gradients are those of the product
+    at the rounded operands, straight through the rounding: x and a float W get dz Q(W) and dz^T Q(x).  `packed` is a packed
+    W (codes, scales) that has no gradient, or None: W is quantised here."""
+
+    @staticmethod
+    def forward(ctx, x, W, packed, b, act, pre, post):
+        wc, ws = packed if packed is not None else _hip.mx_quantize(W.detach())
+        y, slope, mask, xc, xs = _hip.mx_linear_fwd(x.detach(), wc, ws, b, act, pre, post, train=True)
+        ctx.cfg = (act, float(pre), float(post), x.shape[1])
+        ctx.save_for_backward(slope, mask, xc, xs, wc, ws)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        slope, mask, xc, xs, wc, ws = ctx.saved_tensors
+        act, pre, post, K = ctx.cfg
+        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
+        if dy.shape[0] == 0:    # no rows: sums over nothing
+            z = [dy.new_zeros((0, K)), dy.new_zeros((wc.shape[0], K)), dy.new_zeros((wc.shape[0],))]
+            dx, dw, db = (t if n else None for t, n in zip(z, need))
+        else:
+            if dy.stride(1) != 1 or dy.stride(0) < dy.shape[1]:    # expanded or transposed gradients (a sum's, for one)
+                dy = dy.contiguous()
+            dx, dw, db = _hip.mx_linear_bwd(dy, slope, mask, act, pre, post, xc, xs, wc, ws, K, *need)
+        return dx, dw, None, db, None, None, None
+
+
 # ------------------------------------------------------------------------------------------- render
 @custom_op("nerf::render", mutates_args=())
 def render_op(model: int, packed: Tensor, rays_o: Tensor, rays_d: Tensor, t: Tensor, deltas: Tensor, near: float,

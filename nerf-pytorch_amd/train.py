@@ -9,7 +9,9 @@ Extension (no counterpart in the reference): the config key `num_fine_samples = 
 coarse and a fine network with inverse-CDF re-sampling (`num_samples` coarse + N fine samples per
 ray, both losses); checkpoints then hold both networks under `coarse.` / `fine.` key prefixes.
 Extension: the config key `train_precision = bf16x3` (default fp32) runs the training kernels on the bf16
-matrix pipe at fp32 accuracy (three bf16 terms per operand; nerf/models.py set_training_precision).
+matrix pipe at fp32 accuracy (three bf16 terms per operand; nerf/models.py set_training_precision);
+`train_precision = mxfp4` trains a network whose hidden layers run on microscaled 4-bit blocks (single network only),
+which eval.py renders with `--precision mxfp4`.
 """
 import argparse
 import datetime
@@ -81,6 +83,8 @@ def main(argv=None):
     num_fine = int(cfg.get('num_fine_samples', 0))
     if num_fine > 0 and args.optimizer != 'fused':
         raise ValueError("num_fine_samples > 0 (coarse + fine networks) needs --optimizer fused")
+    if num_fine > 0 and cfg.get('train_precision', 'fp32').lower() == 'mxfp4':
+        raise ValueError("train_precision = mxfp4 trains a single network (num_fine_samples = 0)")
     if args.max_iters is not None:
         num_iters = min(num_iters, args.max_iters)
     os.makedirs(save_path, exist_ok=True)
@@ -105,7 +109,9 @@ def main(argv=None):
     train_precision = cfg.get('train_precision', 'fp32').lower()
     if train_precision != 'fp32':
         for net in nets:
-            net.set_training_precision(train_precision)   # raises for anything but 'fp32' / 'bf16x3'
+            net.set_training_precision(train_precision)   # raises for anything but 'fp32' / 'bf16x3' / 'mxfp4'
+            if train_precision == 'mxfp4':
+                net.set_inference_precision('mxfp4')          # validation renders the network that is trained
 
     def render(o, d, us=None, ufs=None):
         """rgb predictions of every network that is trained ([single] or [coarse, fine])."""
