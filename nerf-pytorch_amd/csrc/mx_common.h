@@ -11,7 +11,19 @@
 #pragma once
 #include "common.h"
 
+#include <utility>
+
 namespace mxk {
+
+// f(integral_constant<int, 0>) ... f(integral_constant<int, N-1>)
+template <int... I, typename F>
+__device__ __forceinline__ void unrolled_impl(std::integer_sequence<int, I...>, F&& f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+    unrolled_impl(std::make_integer_sequence<int, N>{}, f);
+}
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));

@@ -133,16 +133,73 @@ __device__ __forceinline__ f32x4 load_bias(const void* bias, int n, int N) {
 
 __device__ __forceinline__ i32x8 wide(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
-// global memory -> LDS, 16 (4) bytes per lane one after the other behind dst; every address lies in [base, base + size).
-// (The size must be a literal for the builtin.)
-__device__ __forceinline__ void load_lds16(const uint8_t* base, int size, uint8_t* dst, int voff, int soff) {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, size, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 16, voff, soff, 0, 0);
+// Rows of an operand as a buffer; global memory -> LDS, 16 (4) bytes per lane one after the other behind dst.  Every
+// address lies in [base, base + size).  (The size must be a literal for the builtin.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* base, int size) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, size, 0x00020000);
 }
-__device__ __forceinline__ void load_lds4(const uint8_t* base, int size, uint8_t* dst, int voff, int soff) {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, size, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 4, voff, soff, 0, 0);
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t b, uint8_t* dst, int voff, int soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)dst, 16, voff, soff, 0, 0);
 }
+__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t b, uint8_t* dst, int voff, int soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)dst, 4, voff, soff, 0, 0);
+}
+
+// Tile of workgroup `t`.  Workgroups go round the eight XCDs; each XCD gets a contiguous run of tiles, walked in groups of
+// eight tile rows, so that what shares an L2 shares operand rows.
+__device__ __forceinline__ void tile_of(const GemmArgs& a, int t, int tm, int tn, int64_t& m0, int& n0) {
+    const int tiles = a.tiles_m * a.tiles_n;
+    const int per = tiles / 8, extra = tiles % 8, xcd = t & 7, i = t >> 3;
+    t = xcd * per + (xcd < extra ? xcd : extra) + i;
+    constexpr int GROUP = 8;
+    const int group = t / (GROUP * a.tiles_n), first = group * GROUP;
+    const int height = a.tiles_m - first < GROUP ? a.tiles_m - first : GROUP;
+    const int in_group = t - group * GROUP * a.tiles_n;
+    m0 = (int64_t)(first + in_group % height) * tm;
+    n0 = in_group / height * tn;
+}
+
+// A wave's sums on their way out, through LDS (32 rows of `lds` at a time): the accumulators hold four n of one m per lane,
+// the stores then take whole rows of the wave's tile.  m, n: the wave tile's place.
+template <int NI, int MI, typename T, int ACT>
+__device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)[NI][MI], float* lds, int64_t m_first, int n_first) {
+    constexpr int WNN = NI * 16, PITCH = WNN + 4;      // floats; 16 bytes of padding spread the rows over the banks
+    constexpr int LPR = WNN / 4, RPI = 64 / LPR;       // lanes per row, rows per instruction
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int n = n_first + (lane % LPR) * 4;
+    const f32x4 bias = a.f.slab ? f32x4{0.f, 0.f, 0.f, 0.f} : load_bias<T>(a.f.bias, n, a.N);
+#pragma unroll
+    for (int jj = 0; jj < MI; jj += 2) {
+#pragma unroll
+        for (int j = jj; j < jj + 2; ++j)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) *reinterpret_cast<f32x4*>(lds + ((j - jj) * 16 + r) * PITCH + i * 16 + q * 4) = acc[i][j];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int row = 0; row < 32; row += RPI) {
+            const int lr = row + lane / LPR;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(lds + lr * PITCH + (lane % LPR) * 4);
+            const int64_t m = m_first + jj * 16 + lr;
+            if (a.f.slab) {
+                float* s = a.f.slab + ((int64_t)blockIdx.z * a.M + m) * a.N + n;
+                if (m < a.M) {
+                    if (n + 4 <= a.N && a.N % 4 == 0) {
+                        *reinterpret_cast<f32x4*>(s) = v;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (n + i < a.N) s[i] = v[i];
+                    }
+                }
+            } else {
+                finish4<T, ACT>(a.f, v, m, n, a.N, m < a.M, bias);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+template <int NI>
+constexpr int store_tile_floats() { return 32 * (NI * 16 + 4); }
 
 // Tile of TM rows x TN columns of the output, WM x WN waves, two LDS stages of 128 bytes a row.
 //
@@ -167,20 +224,9 @@ __global__ __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 1) void mx_gemm_kerne
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
 
-    // Tile of this workgroup.  Workgroups go round the eight XCDs; each XCD gets a contiguous run of tiles, walked in
-    // groups of eight tile rows, so that what shares an L2 shares operand rows.
-    const int tiles = a.tiles_m * a.tiles_n;
-    int t = (int)blockIdx.x;
-    {
-        const int per = tiles / 8, extra = tiles % 8, xcd = t & 7, i = t >> 3;
-        t = xcd * per + (xcd < extra ? xcd : extra) + i;
-    }
-    constexpr int GROUP = 8;
-    const int group = t / (GROUP * a.tiles_n), first = group * GROUP;
-    const int height = a.tiles_m - first < GROUP ? a.tiles_m - first : GROUP;
-    const int in_group = t - group * GROUP * a.tiles_n;
-    const int64_t m0 = (int64_t)(first + in_group % height) * TM;
-    const int n0 = in_group / height * TN;
+    int64_t m0;
+    int n0;
+    tile_of(a, (int)blockIdx.x, TM, TN, m0, n0);
 
     // what this wave stages
     const bool is_w = wave * ROWS < TN;
@@ -216,15 +262,15 @@ __global__ __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 1) void mx_gemm_kerne
         // an odd number of steps: the last stage's second half does not exist; it is read from the first (and not used)
         const bool half = odd && load_st == stages - 1;
         const int back = half && col >= 4 ? 64 : 0;
-        const uint8_t* from = base + load_term * op.plane;
+        const auto rows = buffer_of(base + load_term * op.plane, valid * (int)op.pitch);
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) load_lds16(from, valid * (int)op.pitch, dst + i * 1024, voff[i] - back, load_st * 128);
+        for (int i = 0; i < PIECES; ++i) load_lds16(rows, dst + i * 1024, voff[i] - back, load_st * 128);
         if constexpr (KIND == PACKED) {
             uint8_t* sdst = smem + buf * STAGE + R * 128 + wave * (ROWS * 8);
             const int sback = half && (lane & 1) ? 4 : 0;
+            const auto scales = buffer_of(sbase, valid * (int)op.sc_pitch);
 #pragma unroll
-            for (int i = 0; i < SPIECES; ++i)
-                load_lds4(sbase, valid * (int)op.sc_pitch, sdst + i * 256, svoff[i] - sback, load_st * 8);
+            for (int i = 0; i < SPIECES; ++i) load_lds4(scales, sdst + i * 256, svoff[i] - sback, load_st * 8);
         }
         if (++load_st == stages) { load_st = 0; ++load_term; }
     };
@@ -295,43 +341,236 @@ __global__ __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 1) void mx_gemm_kerne
         if (two) multiply(fr[1]);
     }
 
-    // Out through LDS, two tile rows (32 m) of every wave at a time: the accumulators hold four n of one m per lane, the
-    // stores then take whole rows of the wave's tile.  No request is in flight; the barrier lets the last readers finish.
-    constexpr int WNN = TN / WN, PITCH = WNN + 4;      // floats; 16 bytes of padding spread the rows over the banks
-    constexpr int LPR = WNN / 4, RPI = 64 / LPR;       // lanes per row, rows per instruction
-    static_assert(NW * 32 * PITCH * 4 <= 2 * STAGE, "the way out fits the stages");
+    // no request is in flight; the barrier lets the last readers finish
+    static_assert(NW * store_tile_floats<NI>() * 4 <= 2 * STAGE, "the way out fits the stages");
     __syncthreads();
-    float* out_lds = reinterpret_cast<float*>(smem) + wave * (32 * PITCH);
-    const int n = n0 + wn * WNN + (lane % LPR) * 4;
-    const f32x4 bias = a.f.slab ? f32x4{0.f, 0.f, 0.f, 0.f} : load_bias<T>(a.f.bias, n, a.N);
+    store_tile<NI, MI, T, ACT>(a, acc, reinterpret_cast<float*>(smem) + wave * store_tile_floats<NI>(), m0 + wm * (MI * 16),
+                               n0 + wn * (NI * 16));
+}
+
+// One matrix instruction of the large tile, accumulating IN PLACE in accumulator registers.  With the builtin the compiler
+// takes the result for a new value: it moved the 256 accumulators of the large tile between register files and spilled.
+// What it no longer sees is the result's latency; settle_all() covers that where the sums are read.
+// BYTE: where in their registers the scales are.
+template <int KIND, int BYTE>
+__device__ __forceinline__ void mfma_in_place(f32x4& acc, const i32x4& w, const i32x4& x, int sw, int sx) {
+    static_assert(BYTE < 2, "");
+    if constexpr (KIND == PACKED && BYTE == 0)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                     : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+    else if constexpr (KIND == PACKED)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                     : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+    else
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
+}
+// The wait between the last matrix instructions and the first reads of their results (at most 16 passes of 4 cycles); every
+// accumulator passes through an empty statement behind it, so that no read moves in front.
+template <int NI, int MI>
+__device__ __forceinline__ void settle_all(f32x4 (&acc)[NI][MI]) {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
 #pragma unroll
-    for (int jj = 0; jj < MI; jj += 2) {
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = jj; j < jj + 2; ++j)
+        for (int j = 0; j < MI; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
+
+// The large tile: 256 x 256, four waves of 128 x 128 (one per SIMD: 256 accumulator registers, and per matrix instruction a
+// quarter less LDS traffic than eight waves of 128 x 64).  Stages as above, 128 bytes of each of the 512 rows, in two
+// buffers.  A stage's two halves are 64 matrix instructions each; during the first the second's fragments are read, then
+// -- everybody holds what it needs of this buffer -- comes the stage's one barrier, and during the second half the stage
+// after next is requested into the buffer and the next one's first fragments are read.  The barrier stands in front of
+// matrix instructions whose fragments are in registers, and a request has two halves (2 x 1024 cycles at the full rate) to
+// arrive.  The stream is written out by hand, two matrix instructions and what goes between them at a time; the requests
+// are spread over the whole half, because the four waves' 64 KiB take the vector cache all of it (64 bytes a cycle).
+//
+// PACKED: the order of the blocks inside a stage is free as long as both operands agree, and lane group q takes blocks
+// 2q and 2q + 1 of the eight in its two halves: their two scale bytes are neighbours, one 16-bit read per row and stage,
+// and the matrix instruction picks the byte.  Scales are requested for two stages at a time, 16 bytes a row (8-byte
+// requests of 512 rows cost the L2 as much as the codes did); the last window of a row is moved back to end with it.
+//
+// Rows of 64 bytes a stage in a ring of four (three halves for a request to arrive) were slower: requests of half a cache
+// line halve what the L2 delivers.
+template <int KIND, typename T, int ACT>
+__global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
+    constexpr int TILE = 256, R = 512, NI = 8, MI = 8;
+    constexpr int PIECES = 16;              // requests of a wave per stage
+    constexpr int STAGE = R * 128, SCALES = R * 16;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // two stages; PACKED: and two windows of scales
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4;
+    int64_t m0;
+    int n0;
+    tile_of(a, (int)blockIdx.x, TILE, TILE, m0, n0);
+
+    // waves 0 and 1 stage the tile's 256 rows of W, 2 and 3 those of X; rows behind the last one repeat it (never stored)
+    const bool is_w = wave < 2;
+    const Operand& op = is_w ? a.w : a.x;
+    const int64_t row0 = (is_w ? (int64_t)n0 : m0) + (wave & 1) * 128;
+    const int64_t left = op.rows - row0;
+    const int valid = left > 128 ? 128 : left < 1 ? 1 : (int)left;
+    const int64_t first = left < 1 ? op.rows - 1 : row0;
+    const uint8_t* from = op.p + first * op.pitch;
+    const int size = valid * (int)op.pitch, ssize = valid * (int)op.sc_pitch;
+    const uint8_t* sfrom = KIND == PACKED ? op.sc + first * op.sc_pitch : nullptr;
+    const int col = (lane & 7) ^ (lane >> 3);
+    int voff[PIECES], svoff[2];
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-                *reinterpret_cast<f32x4*>(out_lds + ((j - jj) * 16 + r) * PITCH + i * 16 + q * 4) = acc[i][j];
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int row = 0; row < 32; row += RPI) {
-            const int lr = row + lane / LPR;
-            const f32x4 v = *reinterpret_cast<const f32x4*>(out_lds + lr * PITCH + (lane % LPR) * 4);
-            const int64_t m = m0 + wm * (MI * 16) + jj * 16 + lr;
-            if (a.f.slab) {
-                float* s = a.f.slab + ((int64_t)blockIdx.z * a.M + m) * a.N + n;
-                if (m < a.M) {
-                    if (n + 4 <= a.N && a.N % 4 == 0) *reinterpret_cast<f32x4*>(s) = v;
-                    else
+    for (int i = 0; i < PIECES; ++i) {
+        const int row = i * 8 + (lane >> 3);
+        voff[i] = (row < valid ? row : valid - 1) * (int)op.pitch + col * 16;
+    }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (n + i < a.N) s[i] = v[i];
-                }
-            } else {
-                finish4<T, ACT>(a.f, v, m, n, a.N, m < a.M, bias);
+    for (int i = 0; i < 2; ++i) {
+        const int row = i * 64 + lane;
+        svoff[i] = (row < valid ? row : valid - 1) * (int)op.sc_pitch;
+    }
+    const int stages = (a.steps + 1) / 2;
+    const bool odd = a.steps & 1;     // PACKED, one term: the last stage holds four blocks of eight
+    const int D = stages * a.terms;   // the large tile does not split the reduction
+
+    int load_st = 0;             // stage to request next
+    struct Request {
+        __amdgpu_buffer_rsrc_t rows;
+        uint8_t* dst;
+        int soff;
+    };
+    auto request = [&](int d) {
+        const Request rq{buffer_of(from, size), smem + (d & 1) * STAGE + wave * 16384, load_st * 128};
+        if constexpr (KIND == PACKED) {
+            if ((d & 1) == 0) {
+                const int window = d * 8, end = a.steps * 4 - 16;   // a.steps >= 4
+                const auto rows = buffer_of(sfrom, ssize);
+                uint8_t* dst = smem + 2 * STAGE + (d >> 1 & 1) * SCALES + wave * 2048;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) load_lds16(rows, dst + i * 1024, svoff[i], window < end ? window : end);
+            }
+            if (odd && d == stages - 1) {   // read from the first four blocks instead, and not used (once per tile)
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) voff[i] -= col >= 4 ? 64 : 0;
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        if (++load_st == stages) {
+            load_st = 0;
+            from += op.plane;
+        }
+        return rq;
+    };
+    auto issue = [&](auto I, const Request& rq) { load_lds16(rq.rows, rq.dst + decltype(I)::value * 1024, voff[decltype(I)::value], rq.soff); };
+
+    const int wm = wave >> 1, wn = wave & 1;
+    f32x4 acc[NI][MI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Frags {
+        i32x4 w[NI], x[MI];
+    } f0, f1;
+    struct Scales {
+        int w[NI], x[MI];
+    } scales, next_scales;   // both halves' of a stage
+    const int piece0 = KIND == PACKED ? 2 * q : q, piece1 = KIND == PACKED ? 2 * q + 1 : 4 + q;
+    const int place[2] = {r * 128 + ((piece0 ^ (r & 7)) * 16), r * 128 + ((piece1 ^ (r & 7)) * 16)};
+    const int splace = 2 * STAGE + r * 16 + 2 * q;
+    auto read_one = [&](auto I, auto HALF, Frags& f, const uint8_t* stage, Scales& sc, int scale_at) {   // fragment I of 16: W and X by turns
+        constexpr int i = decltype(I)::value / 2, half = decltype(HALF)::value;
+        if constexpr (decltype(I)::value % 2 == 0) {
+            f.w[i] = *reinterpret_cast<const i32x4*>(stage + wn * 16384 + place[half] + i * 2048);
+            if constexpr (KIND == PACKED && half == 0)
+                sc.w[i] = *reinterpret_cast<const uint16_t*>(smem + splace + scale_at + wn * 2048 + i * 256);
+        } else {
+            f.x[i] = *reinterpret_cast<const i32x4*>(stage + 32768 + wm * 16384 + place[half] + i * 2048);
+            if constexpr (KIND == PACKED && half == 0)
+                sc.x[i] = *reinterpret_cast<const uint16_t*>(smem + splace + scale_at + 4096 + wm * 2048 + i * 256);
+        }
+    };
+    // where the scales of stage d are: their window, and inside it (moved back by what the last window was)
+    auto scales_of = [&](int d) {
+        const int window = (d >> 1) * 16, end = a.steps * 4 - 16;
+        return (d >> 1 & 1) * SCALES + (d & 1) * 8 + (window > end ? window - end : 0);
+    };
+    auto mfma = [&](auto U, auto HALF, const Frags& f) {
+        constexpr int j = decltype(U)::value / NI, i = decltype(U)::value % NI, half = decltype(HALF)::value;
+        mfma_in_place<KIND, half>(acc[i][j], f.w[i], f.x[j], KIND == PACKED ? scales.w[i] : 0, KIND == PACKED ? scales.x[j] : 0);
+    };
+    // the last stage of an odd row: lane groups 2 and 3 multiply zeros (a branch around would put copies of the sums at its end)
+    auto blank = [&](Frags& f) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            f.w[i] = q < 2 ? f.w[i] : i32x4{0, 0, 0, 0};
+            f.x[i] = q < 2 ? f.x[i] : i32x4{0, 0, 0, 0};
+        }
+    };
+    auto publish = [&] {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    constexpr std::integral_constant<int, 0> H0{};
+    constexpr std::integral_constant<int, 1> H1{};
+    // Slot of fragment read k: two of every three slots up to the 24th; of request k: every other slot.
+    constexpr auto read_at = [](int u) { return u < 24 && u % 3 != 2 ? u / 3 * 2 + u % 3 : -1; };
+    // One stage: f0 holds its first half's fragments, and in the end the next stage's.
+    auto stage_body = [&](auto REQUEST, int d) {
+        const uint8_t* here = smem + (d & 1) * STAGE;
+        const uint8_t* next = smem + ((d & 1) ^ 1) * STAGE;
+        if constexpr (!REQUEST)
+            if (KIND == PACKED && odd && d == D - 1) {
+                blank(f0);
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    scales.w[i] = q < 2 ? scales.w[i] : 0;
+                    scales.x[i] = q < 2 ? scales.x[i] : 0;
+                }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        unrolled<32>([&](auto U) {
+            constexpr int u = decltype(U)::value;
+            if constexpr (read_at(u) >= 0) read_one(std::integral_constant<int, read_at(u)>{}, H1, f1, here, scales, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            mfma(std::integral_constant<int, 2 * u>{}, H0, f0);
+            mfma(std::integral_constant<int, 2 * u + 1>{}, H0, f0);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        publish();
+        if constexpr (!REQUEST)
+            if (KIND == PACKED && odd && d == D - 1) blank(f1);
+        Request rq;
+        if constexpr (REQUEST) rq = request(d + 2);
+        const int scale_at = scales_of(d + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        unrolled<32>([&](auto U) {
+            constexpr int u = decltype(U)::value;
+            if constexpr (REQUEST && u % 2 == 0) issue(std::integral_constant<int, u / 2>{}, rq);
+            if constexpr (read_at(u) >= 0) read_one(std::integral_constant<int, read_at(u)>{}, H0, f0, next, next_scales, scale_at);
+            __builtin_amdgcn_sched_barrier(0);
+            mfma(std::integral_constant<int, 2 * u>{}, H1, f1);
+            mfma(std::integral_constant<int, 2 * u + 1>{}, H1, f1);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        scales = next_scales;
+    };
+
+    {
+        const Request rq = request(0);
+        unrolled<PIECES>([&](auto I) { issue(I, rq); });
     }
+    publish();
+    if (D > 1) {
+        const Request rq = request(1);
+        unrolled<PIECES>([&](auto I) { issue(I, rq); });
+    }
+    unrolled<16>([&](auto I) { read_one(I, H0, f0, smem, scales, scales_of(0)); });
+    int d = 0;   // (behind the last stage old contents are read, and not used)
+    for (; d + 2 < D; ++d) stage_body(std::true_type{}, d);
+    for (; d < D; ++d) stage_body(std::false_type{}, d);
+    settle_all(acc);
+    // nothing is under way; the barrier lets the last readers finish
+    static_assert(4 * store_tile_floats<NI>() * 4 <= 2 * STAGE, "the way out fits the stages");
+    __syncthreads();
+    store_tile<NI, MI, T, ACT>(a, acc, reinterpret_cast<float*>(smem) + wave * store_tile_floats<NI>(), m0 + wm * 128, n0 + wn * 128);
 }
 
 // out = finish(sum of the slabs, in their order)
@@ -545,19 +784,23 @@ __global__ __launch_bounds__(256) void mx_turn_kernel(const uint8_t* __restrict_
 constexpr int kTargetGroups = 256;   // compute units
 
 struct Plan {
+    bool large;
     int tiles_m, tiles_n, splits, per_split;
     size_t slab_floats;
 };
 
 // Tile and split of an M x N product over `total` stages.
-Plan plan_for(int64_t M, int64_t N, int64_t total) {
+// steps: 64-byte steps of a row.
+Plan plan_for(int64_t M, int64_t N, int64_t steps, int terms) {
     Plan p{};
-    const int t = 128;
+    const int64_t total = (steps + 1) / 2 * terms;
+    p.large = ceil_div64(M, 256) * ceil_div64(N, 256) >= kTargetGroups * 3 / 4 && steps >= 4;   // (a window of scales is four steps)
+    const int t = p.large ? 256 : 128;
     p.tiles_m = (int)ceil_div64(M, t);
     p.tiles_n = (int)ceil_div64(N, t);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     int64_t splits = 1;
-    if (tiles < kTargetGroups) {
+    if (!p.large && tiles < kTargetGroups) {
         splits = kTargetGroups / tiles;
         const int64_t most = total / 4 < 1 ? 1 : total / 4;    // at least four stages a slice
         if (splits > most) splits = most;
@@ -579,12 +822,21 @@ int launch_gemm_tile(const char* fn, const GemmArgs& a, int splits, hipStream_t 
 }
 
 template <int KIND, typename T, int ACT>
+int launch_gemm_large(const char* fn, const GemmArgs& a, int splits, hipStream_t st) {
+    constexpr int lds = 2 * (512 * 128 + (KIND == PACKED ? 512 * 16 : 0));
+    int rc = nerf_set_lds(mx_gemm_large_kernel<KIND, T, ACT>, lds);
+    if (rc) return rc;
+    mx_gemm_large_kernel<KIND, T, ACT><<<dim3((unsigned)(a.tiles_m * a.tiles_n), 1, (unsigned)splits), 256, lds, st>>>(a);
+    return nerf_check_launch(fn);
+}
+
+template <int KIND, typename T, int ACT>
 int launch_gemm(const char* fn, GemmArgs a, const Plan& p, hipStream_t st) {
     a.tiles_m = p.tiles_m;
     a.tiles_n = p.tiles_n;
     a.per_split = p.per_split;
     if (p.splits == 1) a.f.slab = nullptr;
-    int rc = launch_gemm_tile<KIND, 128, T, ACT>(fn, a, p.splits, st);
+    int rc = p.large ? launch_gemm_large<KIND, T, ACT>(fn, a, p.splits, st) : launch_gemm_tile<KIND, 128, T, ACT>(fn, a, p.splits, st);
     if (rc || p.splits == 1) return rc;
     const int64_t items = a.M * ((a.N + 15) / 16 * 4);
     mx_finish_kernel<T, ACT><<<(unsigned)ceil_div64(items, 256), 256, 0, st>>>(a.f, a.M, a.N, p.splits);
@@ -613,7 +865,7 @@ struct FwdLayout {
 };
 FwdLayout fwd_layout(int64_t M, int64_t K, int64_t N) {
     FwdLayout l{};
-    l.plan = plan_for(M, N, ceil_div64(ceil_div64(K, 128), 2));
+    l.plan = plan_for(M, N, ceil_div64(K, 128), 1);
     l.codes = 0;
     l.scales = up256((size_t)(M * code_pitch(K)));
     l.slab = l.scales + up256((size_t)(M * scale_pitch(K)));
@@ -635,8 +887,8 @@ BwdLayout bwd_layout(int dtype, int act, int64_t M, int64_t K, int64_t N, bool n
     const int64_t tiles = (l.Np / 64) * (l.Mp / 64);
     l.deep = tiles >= 8192 ? 8 : tiles >= 2048 ? 2 : 1;
     l.parts = ceil_div64(l.Mp / 64, l.deep);
-    l.dx = plan_for(M, K, l.Np / 64 * l.terms);
-    l.dw = plan_for(N, K, l.Mp / 64 * l.terms);
+    l.dx = plan_for(M, K, l.Np / 32, l.terms);
+    l.dw = plan_for(N, K, l.Mp / 32, l.terms);
     size_t at = 0;
     l.rows = at;
     if (need_dx) at += up256((size_t)l.terms * M * l.Np * 2);

@@ -166,6 +166,16 @@ def test_linear_shapes(dtype, M, K, N):
     assert torch.equal(mx.linear(x, q, b), y)            # and the same bits again
 
 
+@pytest.mark.parametrize("dtype, act, M, K, N", [
+    (torch.float32, "sin", 3500, 100, 3600), (torch.bfloat16, "none", 3301, 300, 4001), (torch.float16, "relu", 3400, 1030, 3333),
+    (torch.float32, "relu", 50000, 256, 256), (torch.bfloat16, "sigmoid", 12600, 700, 1025), (torch.float16, "none", 130, 513, 100000)])
+def test_linear_many_tiles(dtype, act, M, K, N):
+    """Outputs of some 200 tiles of 256 x 256 and more, one to nine steps along the rows, ragged at both edges."""
+    from nerf import mx
+    x, w, b = randn(M, K, seed=1, dtype=dtype), randn(N, K, seed=2, dtype=dtype, scale=K ** -0.5), randn(N, seed=3, dtype=dtype)
+    check_forward(mx.linear(x, w, b, mx.ACTIVATIONS[act]), x, w, b, act, 1.0, 1.0)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M, K, N", [(1, 300, 50), (40, 200, 70), (700, 256, 256)])
@@ -292,6 +302,18 @@ def test_gradient_activations(dtype, act):
         y, grads = run_training(x, w, b, dy, act, pre, post)
         check_forward(y, x, w, b, act, pre, post)
         check_backward(grads, dy, x, w, b, act, pre, post, dtype)
+
+
+@pytest.mark.parametrize("dtype, act, M, K, N", [
+    (torch.float32, "sin", 3400, 3500, 90), (torch.bfloat16, "none", 3333, 3601, 130), (torch.float16, "sigmoid", 90, 3400, 3600),
+    (torch.float32, "none", 45, 3601, 3400), (torch.bfloat16, "sin", 130, 3400, 3700)])
+def test_gradients_many_tiles(dtype, act, M, K, N):
+    """dx or dW of more than 192 tiles of 256 x 256, one to twelve steps along the reduction."""
+    x, w = randn(M, K, seed=31, dtype=dtype), randn(N, K, seed=32, dtype=dtype, scale=K ** -0.5)
+    b, dy = randn(N, seed=33, dtype=dtype), randn(M, N, seed=34, dtype=dtype)
+    y, grads = run_training(x, w, b, dy, act)
+    check_forward(y, x, w, b, act, 1.0, 1.0)
+    check_backward(grads, dy, x, w, b, act, 1.0, 1.0, dtype)
 
 
 def test_relu_mask_is_the_forward_decision():
