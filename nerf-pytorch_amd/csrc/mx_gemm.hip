@@ -73,10 +73,16 @@ __device__ __forceinline__ void activate(float z, const Finish& f, float& y, flo
     }
 }
 
-// four neighbouring outputs of one row (n .. n+3; `count` of them are inside the row)
-template <typename T, int ACT>
-__device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, int n, int N, bool row_ok, const f32x4& bias) {
-    const int count = N - n;
+// Whether four neighbouring outputs of every row at column n can be stored as one vector (type of the output; fp32).
+template <typename T>
+__device__ __forceinline__ bool whole4(const void* base, int64_t pitch, int n, int N) {
+    return n + 4 <= N && ((uintptr_t)((const T*)base + n) | (uintptr_t)(pitch * sizeof(T))) % (4 * sizeof(T)) == 0;
+}
+
+// Four neighbouring outputs of one row (n .. n+3, those below N); whole: whole4() of the output.  The four lanes that hold
+// sixteen neighbours of one row are a quad, or (ACROSS) sixteen lanes apart.
+template <typename T, int ACT, bool ACROSS>
+__device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, int n, int N, bool row_ok, const f32x4& bias, bool whole) {
     f32x4 y, sl;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -86,35 +92,41 @@ __device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, i
         sl[i] = b;
     }
     if constexpr (ACT == NERF_ACT_RELU) {
-        if (f.mask) {   // uniform; the four lanes of a quad hold sixteen neighbours of one row
+        if (f.mask) {   // uniform
             unsigned bits = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) bits |= (sl[i] > 0.0f && i < count ? 1u : 0u) << i;
-            bits = quad_or(bits << (4 * (threadIdx.x & 3)));
-            if ((threadIdx.x & 3) == 0 && row_ok && count > 0) f.mask[m * ((N + 15) / 16) + n / 16] = (uint16_t)bits;
+            for (int i = 0; i < 4; ++i) bits |= (sl[i] > 0.0f && n + i < N ? 1u : 0u) << i;
+            bits <<= 4 * (n / 4 & 3);
+            if constexpr (ACROSS) {
+                bits |= __shfl_xor(bits, 16);
+                bits |= __shfl_xor(bits, 32);
+            } else {
+                bits = quad_or(bits);
+            }
+            if (n % 16 == 0 && row_ok && n < N) f.mask[m * ((N + 15) / 16) + n / 16] = (uint16_t)bits;
         }
     }
-    if (!row_ok || count <= 0) return;
+    if (!row_ok) return;
     T* o = (T*)f.out + m * f.ldo + n;
     typename Vec<T>::x4 t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] = (T)y[i];
-    if (count >= 4 && ((uintptr_t)o % sizeof(t)) == 0) {
+    if (whole) {
         *reinterpret_cast<typename Vec<T>::x4*>(o) = t;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < count) o[i] = t[i];
+            if (n + i < N) o[i] = t[i];
     }
     if constexpr (ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID) {
         if (f.slope) {
             float* s = f.slope + m * N + n;
-            if (count >= 4 && ((uintptr_t)s % 16) == 0) {
+            if (whole4<float>(f.slope, N, n, N)) {
                 *reinterpret_cast<f32x4*>(s) = sl;
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (i < count) s[i] = sl[i];
+                    if (n + i < N) s[i] = sl[i];
             }
         }
     }
@@ -159,8 +171,31 @@ __device__ __forceinline__ void tile_of(const GemmArgs& a, int t, int tm, int tn
     n0 = in_group / height * tn;
 }
 
-// A wave's sums on their way out, through LDS (32 rows of `lds` at a time): the accumulators hold four n of one m per lane,
-// the stores then take whole rows of the wave's tile.  m, n: the wave tile's place.
+// A wave's sums on their way out as they lie in the registers, four n of one m per lane: rows of 64 bytes (fp32) or 32 at a
+// time, joined in the L2.  For the light activations; half the instructions of the way through LDS, and with one wave per
+// SIMD those are what the end of a tile takes (4096 x 4096: 15 -> 10 us behind the products).
+template <int NI, int MI, typename T, int ACT>
+__device__ __forceinline__ void store_direct(const GemmArgs& a, const f32x4 (&acc)[NI][MI], int64_t m_first, int n_first) {
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    f32x4 bias[NI];
+    bool whole[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        bias[i] = load_bias<T>(a.f.bias, n_first + i * 16 + q * 4, a.N);
+        whole[i] = whole4<T>(a.f.out, a.f.ldo, n_first + i * 16 + q * 4, a.N);
+    }
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int64_t m = m_first + j * 16 + r;
+            finish4<T, ACT, true>(a.f, acc[i][j], m, n_first + i * 16 + q * 4, a.N, m < a.M, bias[i], whole[i]);
+            __builtin_amdgcn_sched_barrier(0);   // one group of registers at a time
+        }
+}
+
+// The same through LDS (32 rows of `lds` at a time): the stores take whole rows of the wave's tile, and the activation's
+// code stands once in a loop.  m, n: the wave tile's place.
 template <int NI, int MI, typename T, int ACT>
 __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)[NI][MI], float* lds, int64_t m_first, int n_first) {
     constexpr int WNN = NI * 16, PITCH = WNN + 4;      // floats; 16 bytes of padding spread the rows over the banks
@@ -168,6 +203,8 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int n = n_first + (lane % LPR) * 4;
     const f32x4 bias = a.f.slab ? f32x4{0.f, 0.f, 0.f, 0.f} : load_bias<T>(a.f.bias, n, a.N);
+    const bool whole = a.f.slab ? whole4<float>(a.f.slab, a.N, n, a.N) : whole4<T>(a.f.out, a.f.ldo, n, a.N);
+    constexpr int U = ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID ? 2 : 8;   // rows in flight
 #pragma unroll
     for (int jj = 0; jj < MI; jj += 2) {
 #pragma unroll
@@ -175,7 +212,7 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)
 #pragma unroll
             for (int i = 0; i < NI; ++i) *reinterpret_cast<f32x4*>(lds + ((j - jj) * 16 + r) * PITCH + i * 16 + q * 4) = acc[i][j];
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
+#pragma unroll U
         for (int row = 0; row < 32; row += RPI) {
             const int lr = row + lane / LPR;
             const f32x4 v = *reinterpret_cast<const f32x4*>(lds + lr * PITCH + (lane % LPR) * 4);
@@ -183,7 +220,7 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)
             if (a.f.slab) {
                 float* s = a.f.slab + ((int64_t)blockIdx.z * a.M + m) * a.N + n;
                 if (m < a.M) {
-                    if (n + 4 <= a.N && a.N % 4 == 0) {
+                    if (whole) {
                         *reinterpret_cast<f32x4*>(s) = v;
                     } else {
 #pragma unroll
@@ -192,7 +229,7 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)
                     }
                 }
             } else {
-                finish4<T, ACT>(a.f, v, m, n, a.N, m < a.M, bias);
+                finish4<T, ACT, false>(a.f, v, m, n, a.N, m < a.M, bias, whole);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -570,7 +607,10 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
     // nothing is under way; the barrier lets the last readers finish
     static_assert(4 * store_tile_floats<NI>() * 4 <= 2 * STAGE, "the way out fits the stages");
     __syncthreads();
-    store_tile<NI, MI, T, ACT>(a, acc, reinterpret_cast<float*>(smem) + wave * store_tile_floats<NI>(), m0 + wm * 128, n0 + wn * 128);
+    if constexpr (ACT == NERF_ACT_NONE || ACT == NERF_ACT_RELU)
+        store_direct<NI, MI, T, ACT>(a, acc, m0 + wm * 128, n0 + wn * 128);
+    else
+        store_tile<NI, MI, T, ACT>(a, acc, reinterpret_cast<float*>(smem) + wave * store_tile_floats<NI>(), m0 + wm * 128, n0 + wn * 128);
 }
 
 // out = finish(sum of the slabs, in their order)
@@ -594,7 +634,7 @@ __global__ __launch_bounds__(256) void mx_finish_kernel(Finish f, int64_t M, int
                     if (n + j < N) v[j] += s[z * step + j];
         }
     }
-    finish4<T, ACT>(f, v, m, n, N, ok, load_bias<T>(f.bias, n, N));
+    finish4<T, ACT, false>(f, v, m, n, N, ok, load_bias<T>(f.bias, n, N), whole4<T>(f.out, f.ldo, n, N));
 }
 
 // ---------------------------------------------------------------------------------------------- gradients: operands
