@@ -262,8 +262,9 @@ int nerf_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, i
 /* y[M,N] = post * f(pre * (Q(x) W^T + b)): x [M,K] is quantised by the call, W [N,K] comes packed, f = NERF_ACT_*, b [N] or
  * NULL; sums in fp32.  For a backward pass the call also writes (NULL to skip): slope [M,N] fp32 = dy/dz for NERF_ACT_SIN
  * and NERF_ACT_SIGMOID; mask [M][ceil(N / 16)] = the decisions of NERF_ACT_RELU, one bit each; xcodes, xscales = the
- * quantised x.  workspace: nerf_mx_linear_fwd_workspace_bytes(M, K, N) bytes, 16-byte aligned. */
-size_t nerf_mx_linear_fwd_workspace_bytes(int64_t M, int64_t K, int64_t N);
+ * quantised x.  workspace: nerf_mx_linear_fwd_workspace_bytes(M, K, N, xcodes != NULL) bytes, 16-byte aligned (NULL where
+ * that is 0). */
+size_t nerf_mx_linear_fwd_workspace_bytes(int64_t M, int64_t K, int64_t N, int keeps_x);
 int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales, const void* bias, int64_t M,
                        int64_t K, int64_t N, int act, double pre, double post, void* y, int64_t ldy, float* slope, uint16_t* mask,
                        uint8_t* xcodes, uint8_t* xscales, void* workspace, void* stream);

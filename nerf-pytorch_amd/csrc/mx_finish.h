@@ -1,0 +1,129 @@
+// How the sums of the MXFP4 products leave: bias, activation, what the backward pass needs, type (mx_gemm.hip, mx_few.hip).
+#pragma once
+#include "mx_common.h"
+#include "sincos.h"
+
+namespace mxk {
+
+// What happens to a sum on its way out.  slab != NULL: fp32 partial sums [split][M][N], finished by mx_finish_kernel.
+struct Finish {
+    void* out;
+    int64_t ldo;
+    const void* bias;       // type of out, or NULL
+    float pre, post;
+    float* slope;           // sin, sigmoid: d y / d z [M][N] for the gradient, or NULL
+    uint16_t* mask;         // relu: decisions [M][ceil(N / 16)], or NULL
+    float* slab;
+};
+
+template <int ACT>
+__device__ __forceinline__ void activate(float z, const Finish& f, float& y, float& slope) {
+    if constexpr (ACT == NERF_ACT_NONE) {
+        y = f.post * f.pre * z;
+        slope = 0.0f;
+    } else if constexpr (ACT == NERF_ACT_RELU) {
+        const float t = f.pre * z;
+        y = f.post * (t <= 0.0f ? 0.0f : t);   // a NaN stays one
+        slope = t > 0.0f ? 1.0f : 0.0f;
+    } else if constexpr (ACT == NERF_ACT_SIN) {
+        float sn, cs;
+        nerf_sincosf(f.pre * z, &sn, &cs);
+        y = f.post * sn;
+        slope = f.post * f.pre * cs;
+    } else {
+        // exp(-|t|) cannot overflow, and 1 - s would cancel: s and 1 - s are both formed from it
+        const float t = f.pre * z, e = expf(-fabsf(t)), r = 1.0f / (1.0f + e);
+        const float s = t >= 0.0f ? r : e * r;
+        y = f.post * (t != t ? t : s);
+        slope = f.post * f.pre * r * (e * r);
+    }
+}
+
+// Whether four neighbouring outputs of every row at column n can be stored as one vector (type of the output; fp32).
+template <typename T>
+__device__ __forceinline__ bool whole4(const void* base, int64_t pitch, int n, int N) {
+    return n + 4 <= N && ((uintptr_t)((const T*)base + n) | (uintptr_t)(pitch * sizeof(T))) % (4 * sizeof(T)) == 0;
+}
+
+// Four neighbouring outputs of one row (n .. n+3, those below N); whole: whole4() of the output.  The four lanes that hold
+// sixteen neighbours of one row are a quad, or (ACROSS) sixteen lanes apart.
+template <typename T, int ACT, bool ACROSS>
+__device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, int n, int N, bool row_ok, const f32x4& bias, bool whole) {
+    f32x4 y, sl;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        activate<ACT>(acc[i] + bias[i], f, a, b);
+        y[i] = a;
+        sl[i] = b;
+    }
+    if constexpr (ACT == NERF_ACT_RELU) {
+        if (f.mask) {   // uniform
+            unsigned bits = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bits |= (sl[i] > 0.0f && n + i < N ? 1u : 0u) << i;
+            bits <<= 4 * (n / 4 & 3);
+            if constexpr (ACROSS) {
+                bits |= __shfl_xor(bits, 16);
+                bits |= __shfl_xor(bits, 32);
+            } else {
+                bits = quad_or(bits);
+            }
+            if (n % 16 == 0 && row_ok && n < N) f.mask[m * ((N + 15) / 16) + n / 16] = (uint16_t)bits;
+        }
+    }
+    if (!row_ok) return;
+    T* o = (T*)f.out + m * f.ldo + n;
+    typename Vec<T>::x4 t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = (T)y[i];
+    if (whole) {
+        *reinterpret_cast<typename Vec<T>::x4*>(o) = t;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < N) o[i] = t[i];
+    }
+    if constexpr (ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID) {
+        if (f.slope) {
+            float* s = f.slope + m * N + n;
+            if (whole4<float>(f.slope, N, n, N)) {
+                *reinterpret_cast<f32x4*>(s) = sl;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < N) s[i] = sl[i];
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 load_bias(const void* bias, int n, int N) {
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < N) b[i] = (float)((const T*)bias)[n + i];
+    }
+    return b;
+}
+
+// Products with few rows (mx_few.hip).  x != NULL: rounded in the kernel (few_fused() says whether that is the way), else
+// xc / xs hold it packed.
+struct FewArgs {
+    const uint8_t *wc, *ws;
+    const void* x;
+    int64_t ldx;
+    bool vec;               // 16-byte loads of x
+    const uint8_t *xc, *xs;
+    int M, K, N;
+    int steps;              // of 128 values
+    Finish f;
+};
+constexpr int kFewRows = 64;
+// One launch for both where every workgroup's rounding of x is short: up to 16384 values.
+static inline bool few_fused(int64_t M, int64_t K) { return M * K <= 16384; }
+int launch_few(const char* fn, const FewArgs& a, int dtype, int act, hipStream_t st);
+
+}  // namespace mxk

@@ -11,8 +11,7 @@
 // rounding of what the previous ones left): one for bf16 dy without a smooth activation (exact), two for fp16 dy (11 bits:
 // exact) and for bf16 dy through sin / sigmoid (2^-17, far under the output's own rounding), three for fp32 (exact up to
 // 2^-25).  Sums are fp32 throughout; a split reduction writes fp32 slabs that a second kernel adds in a fixed order.
-#include "mx_common.h"
-#include "sincos.h"
+#include "mx_finish.h"
 
 namespace mxk {
 namespace {
@@ -28,17 +27,6 @@ struct Operand {
     int64_t plane;          // BF16: bytes between the terms of the operand (0: the same for all terms)
 };
 
-// What happens to a sum on its way out.  slab != NULL: fp32 partial sums [split][M][N], finished by mx_finish_kernel.
-struct Finish {
-    void* out;
-    int64_t ldo;
-    const void* bias;       // type of out, or NULL
-    float pre, post;
-    float* slope;           // sin, sigmoid: d y / d z [M][N] for the gradient, or NULL
-    uint16_t* mask;         // relu: decisions [M][ceil(N / 16)], or NULL
-    float* slab;
-};
-
 struct GemmArgs {
     Operand w, x;           // out[m][n] = sum over steps of x[m] . w[n]
     int64_t M;
@@ -49,99 +37,6 @@ struct GemmArgs {
     int tiles_m, tiles_n;
     Finish f;
 };
-
-template <int ACT>
-__device__ __forceinline__ void activate(float z, const Finish& f, float& y, float& slope) {
-    if constexpr (ACT == NERF_ACT_NONE) {
-        y = f.post * f.pre * z;
-        slope = 0.0f;
-    } else if constexpr (ACT == NERF_ACT_RELU) {
-        const float t = f.pre * z;
-        y = f.post * (t <= 0.0f ? 0.0f : t);   // a NaN stays one
-        slope = t > 0.0f ? 1.0f : 0.0f;
-    } else if constexpr (ACT == NERF_ACT_SIN) {
-        float sn, cs;
-        nerf_sincosf(f.pre * z, &sn, &cs);
-        y = f.post * sn;
-        slope = f.post * f.pre * cs;
-    } else {
-        // exp(-|t|) cannot overflow, and 1 - s would cancel: s and 1 - s are both formed from it
-        const float t = f.pre * z, e = expf(-fabsf(t)), r = 1.0f / (1.0f + e);
-        const float s = t >= 0.0f ? r : e * r;
-        y = f.post * (t != t ? t : s);
-        slope = f.post * f.pre * r * (e * r);
-    }
-}
-
-// Whether four neighbouring outputs of every row at column n can be stored as one vector (type of the output; fp32).
-template <typename T>
-__device__ __forceinline__ bool whole4(const void* base, int64_t pitch, int n, int N) {
-    return n + 4 <= N && ((uintptr_t)((const T*)base + n) | (uintptr_t)(pitch * sizeof(T))) % (4 * sizeof(T)) == 0;
-}
-
-// Four neighbouring outputs of one row (n .. n+3, those below N); whole: whole4() of the output.  The four lanes that hold
-// sixteen neighbours of one row are a quad, or (ACROSS) sixteen lanes apart.
-template <typename T, int ACT, bool ACROSS>
-__device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, int n, int N, bool row_ok, const f32x4& bias, bool whole) {
-    f32x4 y, sl;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float a, b;
-        activate<ACT>(acc[i] + bias[i], f, a, b);
-        y[i] = a;
-        sl[i] = b;
-    }
-    if constexpr (ACT == NERF_ACT_RELU) {
-        if (f.mask) {   // uniform
-            unsigned bits = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) bits |= (sl[i] > 0.0f && n + i < N ? 1u : 0u) << i;
-            bits <<= 4 * (n / 4 & 3);
-            if constexpr (ACROSS) {
-                bits |= __shfl_xor(bits, 16);
-                bits |= __shfl_xor(bits, 32);
-            } else {
-                bits = quad_or(bits);
-            }
-            if (n % 16 == 0 && row_ok && n < N) f.mask[m * ((N + 15) / 16) + n / 16] = (uint16_t)bits;
-        }
-    }
-    if (!row_ok) return;
-    T* o = (T*)f.out + m * f.ldo + n;
-    typename Vec<T>::x4 t;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = (T)y[i];
-    if (whole) {
-        *reinterpret_cast<typename Vec<T>::x4*>(o) = t;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < N) o[i] = t[i];
-    }
-    if constexpr (ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID) {
-        if (f.slope) {
-            float* s = f.slope + m * N + n;
-            if (whole4<float>(f.slope, N, n, N)) {
-                *reinterpret_cast<f32x4*>(s) = sl;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n + i < N) s[i] = sl[i];
-            }
-        }
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ f32x4 load_bias(const void* bias, int n, int N) {
-    f32x4 b = {0.f, 0.f, 0.f, 0.f};
-    if (bias) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < N) b[i] = (float)((const T*)bias)[n + i];
-    }
-    return b;
-}
 
 __device__ __forceinline__ i32x8 wide(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
@@ -900,15 +795,19 @@ int terms_for(int dtype, int act) {
 }
 
 struct FwdLayout {
+    bool few, fused;
     Plan plan;
-    size_t codes, scales, slab, bytes;   // offsets; the quantised x where the caller keeps none
+    size_t scales, slab, bytes;   // offsets (codes at 0): the quantised x where the caller keeps none, partial sums
 };
-FwdLayout fwd_layout(int64_t M, int64_t K, int64_t N) {
+FwdLayout fwd_layout(int64_t M, int64_t K, int64_t N, bool keeps_x) {
     FwdLayout l{};
-    l.plan = plan_for(M, N, ceil_div64(K, 128), 1);
-    l.codes = 0;
-    l.scales = up256((size_t)(M * code_pitch(K)));
-    l.slab = l.scales + up256((size_t)(M * scale_pitch(K)));
+    l.few = M <= kFewRows;
+    l.fused = l.few && !keeps_x && few_fused(M, K);
+    if (!l.few) l.plan = plan_for(M, N, ceil_div64(K, 128), 1);
+    if (!keeps_x && !l.fused) {
+        l.scales = up256((size_t)(M * code_pitch(K)));
+        l.slab = l.scales + up256((size_t)(M * scale_pitch(K)));
+    }
     l.bytes = l.slab + l.plan.slab_floats * 4;
     return l;
 }
@@ -1011,8 +910,8 @@ static bool linear_sizes_ok(int64_t M, int64_t K, int64_t N) {
            ceil_div64(M, 128) * ceil_div64(N, 128) <= (1 << 30);
 }
 
-extern "C" size_t nerf_mx_linear_fwd_workspace_bytes(int64_t M, int64_t K, int64_t N) {
-    return linear_sizes_ok(M, K, N) && M > 0 ? fwd_layout(M, K, N).bytes : 0;
+extern "C" size_t nerf_mx_linear_fwd_workspace_bytes(int64_t M, int64_t K, int64_t N, int keeps_x) {
+    return linear_sizes_ok(M, K, N) && M > 0 ? fwd_layout(M, K, N, keeps_x).bytes : 0;
 }
 
 extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales, const void* bias,
@@ -1028,18 +927,28 @@ extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const u
     NERF_REQUIRE_PTR(wcodes);
     NERF_REQUIRE_PTR(wscales);
     NERF_REQUIRE_PTR(y);
-    NERF_REQUIRE_PTR(workspace);
+    const FwdLayout l = fwd_layout(M, K, N, xcodes != nullptr);
+    if (l.bytes) NERF_REQUIRE_PTR(workspace);
     NERF_REQUIRE((xcodes == nullptr) == (xscales == nullptr), "%s: xcodes and xscales go together", fn);
     NERF_REQUIRE((uintptr_t)wcodes % 16 == 0 && (uintptr_t)wscales % 4 == 0 && (uintptr_t)xcodes % 16 == 0 && (uintptr_t)xscales % 4 == 0 &&
                      (uintptr_t)workspace % 16 == 0,
                  "%s: codes and workspace must be 16-byte, scales 4-byte aligned", fn);
     const hipStream_t st = (hipStream_t)stream;
-    const FwdLayout l = fwd_layout(M, K, N);
     uint8_t* ws = (uint8_t*)workspace;
-    uint8_t* xc = xcodes ? xcodes : ws + l.codes;
+    uint8_t* xc = xcodes ? xcodes : ws;
     uint8_t* xs = xscales ? xscales : ws + l.scales;
-    int rc = launch_quantize(fn, x, dtype, ldx, M, K, xc, xs, st);
-    if (rc) return rc;
+    const Finish f{y, ldy, bias, (float)pre, (float)post, act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID ? slope : nullptr,
+                   act == NERF_ACT_RELU ? mask : nullptr, (float*)(ws + l.slab)};
+    if (!l.fused) {
+        int rc = launch_quantize(fn, x, dtype, ldx, M, K, xc, xs, st);
+        if (rc) return rc;
+    }
+    if (l.few) {
+        const int size = dtype == NERF_F32 ? 4 : 2;
+        const bool vec = (uintptr_t)x % 16 == 0 && ldx * size % 16 == 0;
+        const FewArgs a{wcodes, wscales, l.fused ? x : nullptr, ldx, vec, xc, xs, (int)M, (int)K, (int)N, (int)ceil_div64(K, 128), f};
+        return launch_few(fn, a, dtype, act, st);
+    }
     GemmArgs a{};
     a.w = Operand{wcodes, code_pitch(K), wscales, scale_pitch(K), N, 0};
     a.x = Operand{xc, code_pitch(K), xs, scale_pitch(K), M, 0};
@@ -1047,8 +956,7 @@ extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const u
     a.N = (int)N;
     a.steps = (int)ceil_div64(K, 128);
     a.terms = 1;
-    a.f = Finish{y, ldy, bias, (float)pre, (float)post, act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID ? slope : nullptr,
-                 act == NERF_ACT_RELU ? mask : nullptr, (float*)(ws + l.slab)};
+    a.f = f;
     if (dtype == NERF_F32) return launch_forward<float>(fn, a, l.plan, act, st);
     if (dtype == NERF_BF16) return launch_forward<__bf16>(fn, a, l.plan, act, st);
     return launch_forward<_Float16>(fn, a, l.plan, act, st);

@@ -76,7 +76,7 @@ _SIGS = {
     "nerf_mx_scales_bytes": (c_size_t, [c_int64, c_int64]),
     "nerf_mx_quantize": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, _P, _P]),
     "nerf_mx_dequantize": (c_int, [_P, _P, c_int64, c_int64, c_int, _P, c_int64, _P]),
-    "nerf_mx_linear_fwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "nerf_mx_linear_fwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
     "nerf_mx_linear_fwd": (c_int, [_P, c_int, c_int64, _P, _P, _P, c_int64, c_int64, c_int64, c_int, c_double, c_double, _P, c_int64,
                                    _P, _P, _P, _P, _P, _P]),
     "nerf_mx_linear_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_int]),
@@ -502,28 +502,27 @@ def resample(weights: torch.Tensor, t_coarse: torch.Tensor, u: torch.Tensor, wan
 MX_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _mx_dtype(t: torch.Tensor, name: str) -> int:
-    if t.dtype not in MX_DTYPES:
-        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    return MX_DTYPES[t.dtype]
-
-
 def _mx_rows(t: torch.Tensor, name: str):
-    """(pointer, row pitch in elements) of a matrix whose rows may lie apart but are contiguous themselves."""
+    """(pointer, type, row pitch in elements) of a matrix whose rows may lie apart but are contiguous themselves."""
+    dt = MX_DTYPES.get(t.dtype)
+    if dt is None:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
     if not t.is_cuda:
         raise RuntimeError(f"{name}: tensor is on {t.device}; this build runs on a HIP device only (no CPU path)")
+    if t.is_contiguous() and t.dim() == 2:
+        return t.data_ptr(), dt, t.shape[1]
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         raise ValueError(f"{name}: expected a matrix with contiguous rows that do not overlap")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    return t.data_ptr(), dt, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
 
 
-def _mx_stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _on_device(t: torch.Tensor):
-    """The launches go to the current device: make it the tensor's."""
-    return torch.cuda.device(t.device)
+def _mx_call(fn, index: int, *args) -> int:
+    """fn(*args, stream) with the tensors' device (its index) current and that device's current stream.  These calls are as
+    short as a kernel launch: the device is only switched where it has to be."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def mx_packed_shape(rows: int, K: int):
@@ -532,92 +531,93 @@ def mx_packed_shape(rows: int, K: int):
     return (rows, 64 * blocks), (rows, 4 * blocks)
 
 
-def _mx_packed(codes: torch.Tensor, scales: torch.Tensor, K: int, name: str):
+def _mx_packed(codes: torch.Tensor, scales: torch.Tensor, K: int, device, name: str):
+    """Pointers of packed rows of K values on `device`."""
     c, s = mx_packed_shape(codes.shape[0], K)
-    if tuple(codes.shape) != c or tuple(scales.shape) != s:
+    if codes.shape != c or scales.shape != s:
         raise ValueError(f"{name}: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} are not packed rows of {K} values")
-    if codes.device != scales.device:
-        raise ValueError(f"{name}: codes and scales are on different devices")
+    if codes.device != device or scales.device != device:
+        raise ValueError(f"{name}: codes and scales must be on {device}")
     return _dev(codes, f"{name}.codes", torch.uint8), _dev(scales, f"{name}.scales", torch.uint8)
 
 
-def _mx_alloc(rows: int, K: int, device):
+def _mx_alloc(rows: int, K: int, like: torch.Tensor):
     c, s = mx_packed_shape(rows, K)
-    return torch.empty(c, dtype=torch.uint8, device=device), torch.empty(s, dtype=torch.uint8, device=device)
+    return like.new_empty(c, dtype=torch.uint8), like.new_empty(s, dtype=torch.uint8)
 
 
 def mx_quantize(x: torch.Tensor):
     """x [M,K] -> (codes, scales)."""
-    dt = _mx_dtype(x, "x")
-    ptr, ld = _mx_rows(x, "x")
+    ptr, dt, ld = _mx_rows(x, "x")
     M, K = x.shape
-    with _on_device(x):
-        codes, scales = _mx_alloc(M, K, x.device)
-        _check(lib.nerf_mx_quantize(ptr, dt, ld, M, K, codes.data_ptr(), scales.data_ptr(), _mx_stream(x)), "nerf_mx_quantize")
+    codes, scales = _mx_alloc(M, K, x)
+    rc = _mx_call(lib.nerf_mx_quantize, x.get_device(), ptr, dt, ld, M, K, codes.data_ptr(), scales.data_ptr())
+    if rc:
+        _check(rc, "nerf_mx_quantize")
     return codes, scales
 
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int, dtype) -> torch.Tensor:
-    pc, ps = _mx_packed(codes, scales, K, "packed")
-    if dtype not in MX_DTYPES:
+    pc, ps = _mx_packed(codes, scales, K, codes.device, "packed")
+    dt = MX_DTYPES.get(dtype)
+    if dt is None:
         raise TypeError(f"expected float32, bfloat16 or float16, got {dtype}")
     M = codes.shape[0]
-    with _on_device(codes):
-        out = torch.empty((M, K), dtype=dtype, device=codes.device)
-        _check(lib.nerf_mx_dequantize(pc, ps, M, K, MX_DTYPES[dtype], out.data_ptr(), K, _mx_stream(codes)), "nerf_mx_dequantize")
+    out = codes.new_empty((M, K), dtype=dtype)
+    rc = _mx_call(lib.nerf_mx_dequantize, codes.get_device(), pc, ps, M, K, dt, out.data_ptr(), K)
+    if rc:
+        _check(rc, "nerf_mx_dequantize")
     return out
 
 
 def mx_linear_fwd(x: torch.Tensor, wcodes: torch.Tensor, wscales: torch.Tensor, b: Optional[torch.Tensor], act: int, pre: float,
                   post: float, train: bool = False):
     """y [M,N] = post * f(pre * (Q(x) W^T + b)); with `train` also what the backward needs: (y, slope, mask, xcodes, xscales)."""
-    dt = _mx_dtype(x, "x")
-    ptr, ld = _mx_rows(x, "x")
+    ptr, dt, ld = _mx_rows(x, "x")
     M, K = x.shape
     N = wcodes.shape[0]
-    pc, ps = _mx_packed(wcodes, wscales, K, "weight")
-    if wcodes.device != x.device or (b is not None and b.device != x.device):
-        raise ValueError("mx_linear: x, weight and bias must be on one device")
-    if b is not None and (b.shape != (N,) or b.dtype != x.dtype):
-        raise ValueError(f"mx_linear: bias must be {x.dtype} [{N}], got {b.dtype} {tuple(b.shape)}")
+    pc, ps = _mx_packed(wcodes, wscales, K, x.device, "weight")
+    if b is not None and (b.shape != (N,) or b.dtype != x.dtype or b.device != x.device):
+        raise ValueError(f"mx_linear: bias must be {x.dtype} [{N}] on {x.device}, got {b.dtype} {tuple(b.shape)} on {b.device}")
     slope = mask = xc = xs = None
-    with _on_device(x):
-        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-        if train:
-            if act in (ACT_SIN, ACT_SIGMOID):
-                slope = torch.empty((M, N), dtype=torch.float32, device=x.device)
-            elif act == ACT_RELU:
-                mask = torch.empty((M, (N + 15) // 16), dtype=torch.int16, device=x.device)
-            xc, xs = _mx_alloc(M, K, x.device)
-        ws = torch.empty(lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N), dtype=torch.uint8, device=x.device)
-        ev = timers.start("mx_linear_fwd", M)
-        _check(lib.nerf_mx_linear_fwd(ptr, dt, ld, pc, ps, None if b is None else _dev(b, "b", x.dtype), M, K, N, act, float(pre),
-                                      float(post), y.data_ptr(), N, *(None if t is None else t.data_ptr() for t in (slope, mask, xc, xs)),
-                                      ws.data_ptr(), _mx_stream(x)), "nerf_mx_linear_fwd")
-        timers.stop(ev)
+    y = x.new_empty((M, N))
+    if train:
+        if act in (ACT_SIN, ACT_SIGMOID):
+            slope = x.new_empty((M, N), dtype=torch.float32)
+        elif act == ACT_RELU:
+            mask = x.new_empty((M, (N + 15) // 16), dtype=torch.int16)
+        xc, xs = _mx_alloc(M, K, x)
+    nbytes = lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N, int(train))
+    ws = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    ev = timers.start("mx_linear_fwd", M)
+    rc = _mx_call(lib.nerf_mx_linear_fwd, x.get_device(), ptr, dt, ld, pc, ps, None if b is None else _dev(b, "b", x.dtype), M, K, N, act,
+                  pre, post, y.data_ptr(), N, None if slope is None else slope.data_ptr(), None if mask is None else mask.data_ptr(),
+                  None if xc is None else xc.data_ptr(), None if xs is None else xs.data_ptr(), None if ws is None else ws.data_ptr())
+    if rc:
+        _check(rc, "nerf_mx_linear_fwd")
+    timers.stop(ev)
     return (y, slope, mask, xc, xs) if train else y
 
 
 def mx_linear_bwd(dy: torch.Tensor, slope, mask, act: int, pre: float, post: float, xcodes, xscales, wcodes, wscales, K: int,
                   need_dx: bool, need_dw: bool, need_db: bool):
     """(dx [M,K], dW [N,K], db [N]) in the type of dy, None where not asked for."""
-    dt = _mx_dtype(dy, "dy")
-    ptr, ld = _mx_rows(dy, "dy")
+    ptr, dt, ld = _mx_rows(dy, "dy")
     M, N = dy.shape
-    xp = _mx_packed(xcodes, xscales, K, "x")
-    wp = _mx_packed(wcodes, wscales, K, "weight")
+    xp = _mx_packed(xcodes, xscales, K, dy.device, "x")
+    wp = _mx_packed(wcodes, wscales, K, dy.device, "weight")
     if xcodes.shape[0] != M or wcodes.shape[0] != N:
         raise ValueError(f"mx_linear_bwd: dy {tuple(dy.shape)} does not match x [{xcodes.shape[0]},{K}] and W [{wcodes.shape[0]},{K}]")
-    dev = dy.device
-    with _on_device(dy):
-        dx = torch.empty((M, K), dtype=dy.dtype, device=dev) if need_dx else None
-        dw = torch.empty((N, K), dtype=dy.dtype, device=dev) if need_dw else None
-        db = torch.empty((N,), dtype=dy.dtype, device=dev) if need_db else None
-        ws = torch.empty(lib.nerf_mx_linear_bwd_workspace_bytes(dt, act, M, K, N, need_dx, need_dw, need_db), dtype=torch.uint8, device=dev)
-        ev = timers.start("mx_linear_bwd", M)
-        _check(lib.nerf_mx_linear_bwd(ptr, dt, ld, None if slope is None else slope.data_ptr(), None if mask is None else mask.data_ptr(),
-                                      act, float(pre), float(post), *xp, *wp, M, K, N, ws.data_ptr(),
-                                      None if dx is None else dx.data_ptr(), K, None if dw is None else dw.data_ptr(),
-                                      None if db is None else db.data_ptr(), _mx_stream(dy)), "nerf_mx_linear_bwd")
-        timers.stop(ev)
+    dx = dy.new_empty((M, K)) if need_dx else None
+    dw = dy.new_empty((N, K)) if need_dw else None
+    db = dy.new_empty((N,)) if need_db else None
+    nbytes = lib.nerf_mx_linear_bwd_workspace_bytes(dt, act, M, K, N, need_dx, need_dw, need_db)
+    ws = dy.new_empty((nbytes,), dtype=torch.uint8)
+    ev = timers.start("mx_linear_bwd", M)
+    rc = _mx_call(lib.nerf_mx_linear_bwd, dy.get_device(), ptr, dt, ld, None if slope is None else slope.data_ptr(),
+                  None if mask is None else mask.data_ptr(), act, pre, post, *xp, *wp, M, K, N, ws.data_ptr(),
+                  None if dx is None else dx.data_ptr(), K, None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr())
+    if rc:
+        _check(rc, "nerf_mx_linear_bwd")
+    timers.stop(ev)
     return dx, dw, db

@@ -228,7 +228,7 @@ def test_outputs_beside_the_rows_are_left_alone():
     M, K, N, ld = 37, 160, 45, 64
     x, q = randn(M, K, seed=14), mx.quantize(randn(N, K, seed=15))
     y = torch.full((M, ld), 7.0, device=DEV)
-    ws = torch.empty(_hip.lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N), dtype=torch.uint8, device=DEV)
+    ws = torch.empty(_hip.lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N, 0), dtype=torch.uint8, device=DEV)
     rc = _hip.lib.nerf_mx_linear_fwd(x.data_ptr(), 0, K, q.codes.data_ptr(), q.scales.data_ptr(), None, M, K, N, 0, 1.0, 1.0, y.data_ptr(), ld,
                                      None, None, None, None, ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
     assert rc == 0

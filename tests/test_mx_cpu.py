@@ -36,8 +36,8 @@ def test_sizes():
         assert lib.nerf_mx_codes_bytes(7, K) == 7 * 64 * blocks and lib.nerf_mx_scales_bytes(7, K) == 7 * 4 * blocks
         assert _hip.mx_packed_shape(7, K) == ((7, 64 * blocks), (7, 4 * blocks))
     assert lib.nerf_mx_codes_bytes(-1, 8) == 0 and lib.nerf_mx_codes_bytes(8, 0) == 0 and lib.nerf_mx_scales_bytes(8, 1 << 23) == 0
-    assert lib.nerf_mx_linear_fwd_workspace_bytes(0, 8, 8) == 0 and lib.nerf_mx_linear_fwd_workspace_bytes(8, 0, 8) == 0
-    assert lib.nerf_mx_linear_fwd_workspace_bytes(1 << 31, 8, 8) == 0
+    assert lib.nerf_mx_linear_fwd_workspace_bytes(0, 8, 8, 0) == 0 and lib.nerf_mx_linear_fwd_workspace_bytes(8, 0, 8, 0) == 0
+    assert lib.nerf_mx_linear_fwd_workspace_bytes(1 << 31, 8, 8, 0) == 0
     assert lib.nerf_mx_linear_bwd_workspace_bytes(9, 0, 8, 8, 8, 1, 1, 1) == 0
     assert lib.nerf_mx_linear_bwd_workspace_bytes(0, 0, 0, 8, 8, 1, 1, 1) == 0
     assert lib.nerf_mx_linear_bwd_workspace_bytes(0, 0, 64, 64, 64, 0, 0, 0) == 0
@@ -86,7 +86,7 @@ def _fwd(**kw):
 
 @pytest.mark.parametrize("kw, code, text", [
     (dict(x=None), -2, b"x is NULL"), (dict(wc=None), -2, b"wcodes is NULL"), (dict(ws=None), -2, b"wscales is NULL"),
-    (dict(y=None), -2, b"y is NULL"), (dict(work=None), -2, b"workspace is NULL"),
+    (dict(y=None), -2, b"y is NULL"), (dict(work=None, M=200), -2, b"workspace is NULL"),
     (dict(ldx=31), -1, b"ldx=31"), (dict(ldy=7), -1, b"ldy=7"), (dict(dtype=5), -1, b"unknown type 5"),
     (dict(act=4), -1, b"unknown activation 4"), (dict(M=-1), -1, b"M=-1"), (dict(K=0), -1, b"K=0"), (dict(N=0), -1, b"N=0"),
     (dict(M=(1 << 30) + 1), -1, b"bad shape"), (dict(K=(1 << 22) + 1, ldx=1 << 23), -1, b"bad shape"),
