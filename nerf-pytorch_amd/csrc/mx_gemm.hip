@@ -11,7 +11,7 @@
 // rounding of what the previous ones left): one for bf16 dy without a smooth activation (exact), two for fp16 dy (11 bits:
 // exact) and for bf16 dy through sin / sigmoid (2^-17, far under the output's own rounding), three for fp32 (exact up to
 // 2^-25).  Sums are fp32 throughout; a split reduction writes fp32 slabs that a second kernel adds in a fixed order.
-#include "mx_finish.h"
+#include "mx_narrow.h"
 
 namespace mxk {
 namespace {
@@ -795,15 +795,16 @@ int terms_for(int dtype, int act) {
 }
 
 struct FwdLayout {
-    bool few, fused;
+    bool few, narrow, fused;      // fused: x is rounded by the product's own kernel
     Plan plan;
     size_t scales, slab, bytes;   // offsets (codes at 0): the quantised x where the caller keeps none, partial sums
 };
 FwdLayout fwd_layout(int64_t M, int64_t K, int64_t N, bool keeps_x) {
     FwdLayout l{};
     l.few = M <= kFewRows;
-    l.fused = l.few && !keeps_x && few_fused(M, K);
-    if (!l.few) l.plan = plan_for(M, N, ceil_div64(K, 128), 1);
+    l.narrow = M >= kNarrowRows && K <= kNarrow && N <= kNarrow;
+    l.fused = (l.few && !keeps_x && few_fused(M, K)) || l.narrow;
+    if (!l.few && !l.narrow) l.plan = plan_for(M, N, ceil_div64(K, 128), 1);
     if (!keeps_x && !l.fused) {
         l.scales = up256((size_t)(M * code_pitch(K)));
         l.slab = l.scales + up256((size_t)(M * scale_pitch(K)));
@@ -939,6 +940,10 @@ extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const u
     uint8_t* xs = xscales ? xscales : ws + l.scales;
     const Finish f{y, ldy, bias, (float)pre, (float)post, act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID ? slope : nullptr,
                    act == NERF_ACT_RELU ? mask : nullptr, (float*)(ws + l.slab)};
+    if (l.narrow) {
+        const NarrowFwd a{x, ldx, M, (int)K, (int)N, wcodes, wscales, xcodes, xscales, false, false, f};
+        return launch_narrow_fwd(fn, a, dtype, act, st);
+    }
     if (!l.fused) {
         int rc = launch_quantize(fn, x, dtype, ldx, M, K, xc, xs, st);
         if (rc) return rc;

@@ -176,6 +176,24 @@ def test_linear_many_tiles(dtype, act, M, K, N):
     check_forward(mx.linear(x, w, b, mx.ACTIVATIONS[act]), x, w, b, act, 1.0, 1.0)
 
 
+NARROW = [(4096, 256, 256), (4111, 100, 33), (4097, 31, 16), (6001, 255, 250), (4500, 132, 1), (5003, 128, 129), (9000, 64, 64), (4099, 1, 200)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M, K, N", NARROW)
+def test_linear_narrow(dtype, act, M, K, N):
+    """Up to 256 inputs and outputs over many rows, ragged everywhere; then rows with a pitch and at an odd address."""
+    from nerf import mx
+    x, w, b = randn(M, K, seed=1, dtype=dtype), randn(N, K, seed=2, dtype=dtype, scale=K ** -0.5), randn(N, seed=3, dtype=dtype)
+    y = mx.linear(x, w, b, mx.ACTIVATIONS[act], 1.5, 2.0)
+    check_forward(y, x, w, b, act, 1.5, 2.0)
+    buf = randn(M * (K + 8) + 5, seed=4, dtype=dtype)
+    for shift, width in ((0, K + 8), (5, K + 3)):
+        x2 = buf[shift:shift + M * width].view(M, width)[:, :K]
+        assert torch.equal(mx.linear(x2, w, b, mx.ACTIVATIONS[act]), mx.linear(x2.contiguous(), w, b, mx.ACTIVATIONS[act]))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M, K, N", [(1, 300, 50), (40, 200, 70), (700, 256, 256)])
@@ -302,6 +320,20 @@ def test_gradient_activations(dtype, act):
         y, grads = run_training(x, w, b, dy, act, pre, post)
         check_forward(y, x, w, b, act, pre, post)
         check_backward(grads, dy, x, w, b, act, pre, post, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M, K, N", NARROW)
+def test_gradients_narrow(dtype, act, M, K, N):
+    x, w = randn(M, K, seed=31, dtype=dtype), randn(N, K, seed=32, dtype=dtype, scale=K ** -0.5)
+    b = (torch.sign(randn(N, seed=33)) * 30).to(dtype) if act == "relu" else randn(N, seed=33, dtype=dtype)
+    dy = randn(M, N, seed=34, dtype=dtype)
+    y, grads = run_training(x, w, b, dy, act, 1.5, 2.0)
+    check_forward(y, x, w, b, act, 1.5, 2.0)
+    check_backward(grads, dy, x, w, b, act, 1.5, 2.0, dtype)
+    again = run_training(x, w, b, torch.cat([dy, dy], 1)[:, N:], act, 1.5, 2.0)[1]      # dy with a pitch
+    assert all(torch.equal(a, c) for a, c in zip(grads, again))
 
 
 @pytest.mark.parametrize("dtype, act, M, K, N", [
