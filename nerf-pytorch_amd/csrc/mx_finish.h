@@ -109,6 +109,19 @@ __device__ __forceinline__ f32x4 load_bias(const void* bias, int n, int N) {
     return b;
 }
 
+// A value as bf16 terms, v = t0 + t1 + ..: each the rounding of what the previous ones left.
+template <int TERMS>
+__device__ __forceinline__ void split_terms(float v, __bf16 (&t)[TERMS]) {
+    const float top = __builtin_bit_cast(float, 0x7f7f0000u);   // largest bf16: fp32 values above it would round to infinity
+    const bool finite = fabsf(v) < __builtin_inff();
+    t[0] = (__bf16)(finite ? fminf(fmaxf(v, -top), top) : v);
+#pragma unroll
+    for (int i = 1; i < TERMS; ++i) {
+        v = finite ? v - (float)t[i - 1] : 0.0f;                // exact
+        t[i] = (__bf16)v;
+    }
+}
+
 // Products with few rows (mx_few.hip).  x != NULL: rounded in the kernel (few_fused() says whether that is the way), else
 // xc / xs hold it packed.
 struct FewArgs {

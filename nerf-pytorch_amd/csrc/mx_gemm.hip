@@ -536,18 +536,6 @@ __global__ __launch_bounds__(256) void mx_finish_kernel(Finish f, int64_t M, int
 // dz = dy * (d y / d z), split into bf16 terms: rows [term][M][Np] for the data gradient and, turned, [term][N][Mp] for
 // the weight gradient (either may be NULL); Np, Mp: rounded up to 64, zeros behind the end.  colsum: partial column sums
 // of dz [grid.y][N], or NULL.  Tiles of 64 x 64 through LDS, `deep` of them one under the other per workgroup.
-template <int TERMS>
-__device__ __forceinline__ void split_terms(float v, __bf16 (&t)[TERMS]) {
-    const float top = __builtin_bit_cast(float, 0x7f7f0000u);   // largest bf16: fp32 values above it would round to infinity
-    const bool finite = fabsf(v) < __builtin_inff();
-    t[0] = (__bf16)(finite ? fminf(fmaxf(v, -top), top) : v);
-#pragma unroll
-    for (int i = 1; i < TERMS; ++i) {
-        v = finite ? v - (float)t[i - 1] : 0.0f;                // exact
-        t[i] = (__bf16)v;
-    }
-}
-
 struct DzArgs {
     const void* dy;
     int64_t lddy;
@@ -814,13 +802,23 @@ FwdLayout fwd_layout(int64_t M, int64_t K, int64_t N, bool keeps_x) {
 }
 
 struct BwdLayout {
+    bool narrow;
     int terms, deep;
     int64_t Np, Mp, parts;
     Plan dx, dw;
     size_t rows, turned, part, wt, xt, slab, bytes;
 };
-BwdLayout bwd_layout(int dtype, int act, int64_t M, int64_t K, int64_t N, bool need_dx, bool need_dw, bool need_db) {
+// `narrow`: whether the layout of dy allows that path; the size that callers ask for covers both ways.
+BwdLayout bwd_layout(int dtype, int act, int64_t M, int64_t K, int64_t N, bool need_dx, bool need_dw, bool need_db, bool narrow) {
     BwdLayout l{};
+    if (narrow) {
+        l.narrow = true;
+        const int groups = narrow_groups(M), c = narrow_columns(K, N);
+        if (need_dw) l.bytes = (size_t)groups * c * c * 4;
+        l.part = l.bytes;
+        if (need_db) l.bytes += up256((size_t)groups * N * 4);
+        return l;
+    }
     l.terms = terms_for(dtype, act);
     l.Np = ceil_div64(N, 64) * 64;
     l.Mp = ceil_div64(M, 64) * 64;
@@ -856,6 +854,14 @@ int launch_dz(const char* fn, const DzArgs& a, int terms, hipStream_t st) {
     return nerf_check_launch(fn);
 }
 
+int launch_colsum(const char* fn, const float* part, int parts, int N, int dtype, void* db, hipStream_t st) {
+    const unsigned grid = (unsigned)ceil_div64(N, 16);
+    if (dtype == NERF_F32) mx_colsum_kernel<float><<<grid, 256, 0, st>>>(part, parts, N, (float*)db);
+    else if (dtype == NERF_BF16) mx_colsum_kernel<__bf16><<<grid, 256, 0, st>>>(part, parts, N, (__bf16*)db);
+    else mx_colsum_kernel<_Float16><<<grid, 256, 0, st>>>(part, parts, N, (_Float16*)db);
+    return nerf_check_launch(fn);
+}
+
 template <typename T>
 int backward(const char* fn, const BwdLayout& l, DzArgs dz, const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes,
              const uint8_t* wscales, int64_t M, int64_t K, int64_t N, uint8_t* ws, void* dx, int64_t lddx, void* dw, void* db,
@@ -865,10 +871,8 @@ int backward(const char* fn, const BwdLayout& l, DzArgs dz, const uint8_t* xcode
     dz.colsum = db ? (float*)(ws + l.part) : nullptr;
     int rc = launch_dz<T>(fn, dz, l.terms, st);
     if (rc) return rc;
-    if (db) {
-        mx_colsum_kernel<T><<<(unsigned)ceil_div64(N, 16), 256, 0, st>>>(dz.colsum, (int)l.parts, (int)N, (T*)db);
-        if ((rc = nerf_check_launch(fn))) return rc;
-    }
+    constexpr int dtype = sizeof(T) == 4 ? NERF_F32 : __is_same(T, __bf16) ? NERF_BF16 : NERF_F16;
+    if (db && (rc = launch_colsum(fn, dz.colsum, (int)l.parts, (int)N, dtype, db, st))) return rc;
     if (dx) {   // dx[m][k] = sum over n of dz[m][n] W[n][k]
         mx_turn_kernel<<<dim3((unsigned)ceil_div64(K, 128), (unsigned)(l.Np / 64)), 256, 0, st>>>(wcodes, wscales, N, K, l.Np,
                                                                                                  (__bf16*)(ws + l.wt));
@@ -970,7 +974,10 @@ extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const u
 extern "C" size_t nerf_mx_linear_bwd_workspace_bytes(int dtype, int act, int64_t M, int64_t K, int64_t N, int need_dx, int need_dw,
                                                      int need_db) {
     if (!linear_sizes_ok(M, K, N) || M < 1 || dtype < NERF_F32 || dtype > NERF_F16) return 0;
-    return bwd_layout(dtype, act, M, K, N, need_dx, need_dw, need_db).bytes;
+    const size_t general = bwd_layout(dtype, act, M, K, N, need_dx, need_dw, need_db, false).bytes;
+    if (M < kNarrowRows || K > kNarrow || N > kNarrow) return general;
+    const size_t narrow = bwd_layout(dtype, act, M, K, N, need_dx, need_dw, need_db, true).bytes;
+    return narrow > general ? narrow : general;
 }
 
 extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const float* slope, const uint16_t* mask, int act, double pre,
@@ -992,11 +999,14 @@ extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const
     if (dw) { NERF_REQUIRE_PTR(xcodes); NERF_REQUIRE_PTR(xscales); }
     NERF_REQUIRE((uintptr_t)wcodes % 16 == 0 && (uintptr_t)xcodes % 16 == 0 && (uintptr_t)workspace % 16 == 0,
                  "%s: codes and workspace must be 16-byte aligned", fn);
-    const BwdLayout l = bwd_layout(dtype, act, M, K, N, dx != nullptr, dw != nullptr, db != nullptr);
+    const bool smooth = act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID;
+    const int size = dtype == NERF_F32 ? 4 : 2;
+    const BwdLayout l = bwd_layout(dtype, act, M, K, N, dx != nullptr, dw != nullptr, db != nullptr,
+                                   narrow_bwd_ok(dy, lddy, size, M, K, N, smooth ? slope : nullptr));
     DzArgs dz{};
     dz.dy = dy;
     dz.lddy = lddy;
-    dz.slope = act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID ? slope : nullptr;
+    dz.slope = smooth ? slope : nullptr;
     dz.mask = act == NERF_ACT_RELU ? mask : nullptr;
     // the constant factor of dz stays out of the terms (they are exact without it) and is applied to the sums
     dz.factor = dz.slope ? 1.0f : (float)(pre * post);
@@ -1007,6 +1017,12 @@ extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const
     dz.deep = l.deep;
     const hipStream_t st = (hipStream_t)stream;
     uint8_t* ws = (uint8_t*)workspace;
+    if (l.narrow) {
+        float* part = db ? (float*)(ws + l.part) : nullptr;
+        const NarrowBwd a{dy, lddy, dz.slope, dz.mask, dz.factor, xcodes, xscales, wcodes, wscales, M, (int)K, (int)N, dx, lddx, dw, (float*)ws, part, false};
+        int rc = launch_narrow_bwd(fn, a, dtype, st);
+        return rc || !db ? rc : launch_colsum(fn, part, narrow_groups(M), (int)N, dtype, db, st);
+    }
     if (dtype == NERF_F32)
         return backward<float>(fn, l, dz, xcodes, xscales, wcodes, wscales, M, K, N, ws, dx, lddx, dw, db, st);
     if (dtype == NERF_BF16)

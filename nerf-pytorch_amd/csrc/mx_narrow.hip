@@ -150,7 +150,331 @@ int by_act(const char* fn, NarrowFwd a, int act, hipStream_t st) {
     return by_steps<T, NERF_ACT_SIGMOID>(fn, a, st);
 }
 
+// ------------------------------------------------------------------------------------------------------- backward
+// All three gradients in one pass over dy, the slopes and the packed x.  A workgroup of eight waves walks its 32-row pieces:
+//   * dy, slopes and codes of the next piece come straight into LDS while this one is multiplied;
+//   * dz = dy * slope is split into bf16 terms, x is decoded, both as rows in LDS;
+//   * dx: the 32 rows times W, whose fragments every wave keeps in registers (an eighth of the columns each);
+//   * dW += dz^T x: each wave keeps a quarter by a half of the whole C x C result in accumulators to the end; the operands
+//     run along the rows here, so they are read with the transposing LDS read (ds_read_b64_tr_b16: lane j of sixteen gets
+//     column j of four rows);
+//   * db: column sums in registers.
+// In the end every workgroup writes its dW and db sums, two small kernels add them in order.  262144 x 256 x 256 fp32 moves
+// 0.84 GB; ROUNDED.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);   // addresses are clamped by hand
+}
+__device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t b, uint8_t* dst, int voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)dst, 16, voff, 0, 0, 0);
+}
+__device__ __forceinline__ void to_lds4(__amdgpu_buffer_rsrc_t b, uint8_t* dst, int voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)dst, 4, voff, 0, 0, 0);
+}
+// eight rows of a column: `at` is this lane's place for four of them, the other four lie `four` bytes on
+__device__ __forceinline__ bf16x8 read_turned(const uint8_t* at, int four) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + four));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Sums over the four 16-lane rows of a wave of four values each: row i of the result holds value i's sum.
+__device__ __forceinline__ float rows_sum(float a, float b, float c, float d) {
+    const auto add = [](unsigned x, unsigned y) { return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y); };
+    const auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
+    const auto p = __builtin_amdgcn_permlane16_swap(bits(a), bits(b), false, false);    // rows 0, 2 of the sum: a, rows 1, 3: b
+    const auto s = __builtin_amdgcn_permlane16_swap(bits(c), bits(d), false, false);
+    const unsigned ab = bits(add(p[0], p[1])), cd = bits(add(s[0], s[1]));
+    const auto v = __builtin_amdgcn_permlane32_swap(ab, cd, false, false);
+    return add(v[0], v[1]);
+}
+
+template <typename T, int TERMS, int C>
+struct NarrowLds {
+    static constexpr int PITCH = C * 2 + 32;                  // bytes of a row of bf16; 32 of padding spread rows over the banks
+    static constexpr int PLANE = 32 * PITCH;
+    static constexpr int X = TERMS * PLANE;                   // decoded x behind the terms of dz
+    static constexpr int DY = X + PLANE, SLOPE = DY + 32 * C * (int)sizeof(T), CODES = SLOPE + 32 * C * 4, SCALES = CODES + 32 * C / 2;
+    static constexpr int BYTES = SCALES + 256;
+};
+
+// SLOPE: 0 none, 1 slopes, 2 decisions of a ReLU.
+template <typename T, int TERMS, int C, int SLOPE>
+__global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
+    using L = NarrowLds<T, TERMS, C>;
+    constexpr int PITCH = L::PITCH, STEPS = C / 128;
+    constexpr int NT = C / 64, KT = C / 32, XT = C / 128;     // tiles of a wave: dW (NT of n, KT of k), dx (XT of k)
+    constexpr int CHUNKS = C / 64;                            // groups of four columns a thread converts
+    constexpr int CODES = C / 16;                             // codes a thread decodes
+    typedef T x4 __attribute__((ext_vector_type(4)));
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, q = lane >> 4;
+    const int steps = (a.K + 127) / 128;
+    const int row = tid >> 4, l16 = tid & 15;                 // what this thread converts
+    const int64_t pieces = (a.M + 31) / 32;
+    const int turned = (q * 8 + (r >> 2)) * PITCH + (r & 3) * 8;   // this lane's place in a 32 x 16 block read turned
+
+    // codes of one row -> bf16 values in LDS
+    auto decode = [&](const uint8_t* codes, unsigned s, bool in) {
+        uint8_t* o = smem + L::X + row * PITCH + l16 * (CODES * 2);
+#pragma unroll
+        for (int i = 0; i < CODES / 8; ++i) {
+            const unsigned c = reinterpret_cast<const unsigned*>(codes)[i];
+            *reinterpret_cast<bf16x8*>(o + i * 16) = in ? decode8_bf16(c, s) : decode8_bf16(0u, 0u);
+        }
+    };
+
+    // this wave's columns of W, as the A operand of dx = dz W: 32 rows of W at a time through LDS
+    bf16x8 wf[XT][C / 32];
+    if (a.dx) {
+#pragma unroll
+        for (int s = 0; s < C / 32; ++s) {
+            const int n = s * 32 + row, k = l16 * CODES;
+            const bool in = n < a.N && k < steps * 128;
+            const int64_t at = in ? (int64_t)n * (steps * 128) + k : 0;    // values from the first code
+            decode(a.wc + at / 2, a.ws[at / 32], in);
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < XT; ++t) wf[t][s] = read_turned(smem + L::X + turned + (wave * XT + t) * 32, 4 * PITCH);
+            __syncthreads();
+        }
+    }
+
+    constexpr int DYB = C * (int)sizeof(T), DYN = 32 * DYB / 1024, SLN = 32 * C * 4 / 1024, CON = 32 * C / 2 / 1024;
+    [[maybe_unused]] uint16_t bits[CHUNKS];
+    auto request = [&](int64_t piece) {
+        // (hidden from the compiler, which would keep every lane's offsets in registers across the loop)
+        int lane = threadIdx.x & 63, row = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+        asm volatile("" : "+v"(lane), "+v"(row), "+v"(l16));
+        const int64_t m0 = piece * 32;
+        const int rows = a.M - m0 < 32 ? (int)(a.M - m0) : 32;
+        auto clamp = [&](int v) { return v < rows ? v : rows - 1; };
+        const auto dy = rows_of((const T*)a.dy + m0 * a.lddy);
+#pragma unroll
+        for (int i = 0; i < (DYN + 7) / 8; ++i) {
+            const int p = i * 8 + wave;
+            if (DYN % 8 == 0 || p < DYN) {
+                const int byte = p * 1024 + lane * 16, c = byte % DYB;
+                to_lds16(dy, smem + L::DY + p * 1024, clamp(byte / DYB) * (int)a.lddy * (int)sizeof(T) + (c < a.N * (int)sizeof(T) ? c : 0));
+            }
+        }
+        if constexpr (SLOPE == 1) {
+            const auto sl = rows_of(a.slope + m0 * a.N);
+#pragma unroll
+            for (int i = 0; i < (SLN + 7) / 8; ++i) {
+                const int p = i * 8 + wave, byte = p * 1024 + lane * 16, c = byte % (C * 4);
+                to_lds16(sl, smem + L::SLOPE + p * 1024, clamp(byte / (C * 4)) * a.N * 4 + (c < a.N * 4 ? c : 0));
+            }
+        }
+        if (a.dw && wave < CON + 1) {
+            if (wave < CON) {
+                const int byte = wave * 1024 + lane * 16, c = byte % (C / 2);
+                to_lds16(rows_of(a.xc + m0 * (steps * 64)), smem + L::CODES + wave * 1024,
+                         clamp(byte / (C / 2)) * (steps * 64) + (c < steps * 64 ? c : 0));
+            } else {
+                const int byte = lane * 4, c = byte % (C / 32);      // C = 128: the upper lanes repeat rows, behind what is read
+                to_lds4(rows_of(a.xs + m0 * (steps * 4)), smem + L::SCALES, clamp(byte / (C / 32) % 32) * (steps * 4) + (c < steps * 4 ? c : 0));
+            }
+        }
+        if constexpr (SLOPE == 2) {
+            const int words = (a.N + 15) / 16;
+#pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) {
+                const int w = i * 4 + l16 / 4;
+                bits[i] = w < words ? a.mask[(m0 + clamp(row)) * words + w] : 0;
+            }
+        }
+    };
+
+    f32x4 acc[KT][NT];
+#pragma unroll
+    for (int i = 0; i < KT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 db = {0.f, 0.f, 0.f, 0.f};     // lane row q: columns 64 q + 4 l16 ..
+    const int wn = wave >> 1, wk = wave & 1;
+
+    int64_t piece = blockIdx.x;
+    if (piece < pieces) request(piece);
+    for (; piece < pieces; piece += gridDim.x) {
+        // the piece has landed, and everybody is done with the rows of the previous one
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        int row = threadIdx.x >> 4, l16 = threadIdx.x & 15, r = lane & 15, q = lane >> 4;    // (hidden as above)
+        asm volatile("" : "+v"(row), "+v"(l16), "+v"(r), "+v"(q));
+        const int64_t m0 = piece * 32;
+        const bool in_row = m0 + row < a.M;
+        f32x4 dz[4] = {};
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            const int n = i * 64 + l16 * 4;
+            const x4 d = *reinterpret_cast<const x4*>(smem + L::DY + row * DYB + n * (int)sizeof(T));
+            f32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = in_row && n < a.N ? (float)d[j] : 0.0f;      // N is a multiple of four
+            if constexpr (SLOPE == 1) {
+                const f32x4 s = *reinterpret_cast<const f32x4*>(smem + L::SLOPE + row * (C * 4) + n * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = in_row && n < a.N ? v[j] * s[j] : 0.0f;
+            }
+            if constexpr (SLOPE == 2) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = bits[i] >> (4 * (l16 & 3) + j) & 1 ? v[j] : 0.0f;
+            }
+            __bf16 t[4][TERMS];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split_terms<TERMS>(v[j], t[j]);
+            dz[i] = v;
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k)
+                *reinterpret_cast<bf16x4*>(smem + k * L::PLANE + row * PITCH + n * 2) = bf16x4{t[0][k], t[1][k], t[2][k], t[3][k]};
+            __builtin_amdgcn_sched_barrier(0);      // registers are short: one group at a time
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) db[j] += rows_sum(dz[0][j], dz[1][j], dz[2][j], dz[3][j]);
+        if (a.dw) {
+            const int k = l16 * CODES;
+            decode(smem + L::CODES + row * (C / 2) + k / 2, smem[L::SCALES + row * (C / 32) + k / 32], in_row && k < steps * 128);
+        }
+        __syncthreads();
+        if (piece + gridDim.x < pieces) request(piece + gridDim.x);
+
+        if (a.dx) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                f32x4 o[XT];
+#pragma unroll
+                for (int t = 0; t < XT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < C / 32; ++s) {
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) {
+                        const bf16x8 z = *reinterpret_cast<const bf16x8*>(smem + k * L::PLANE + (mt * 16 + r) * PITCH + s * 64 + q * 16);
+#pragma unroll
+                        for (int t = 0; t < XT; ++t) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[t][s], z, o[t], 0, 0, 0);
+                    }
+                    if (s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                }
+                const int64_t m = m0 + mt * 16 + r;
+                if (m < a.M) {
+#pragma unroll
+                    for (int t = 0; t < XT; ++t) {
+                        const int k = (wave * XT + t) * 16 + q * 4;
+                        T* p = (T*)a.dx + m * a.lddx + k;
+                        x4 v;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = (T)(o[t][j] * a.factor);
+                        if (a.whole && k + 4 <= a.K) {
+                            *reinterpret_cast<x4*>(p) = v;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (k + j < a.K) p[j] = v[j];
+                        }
+                    }
+                }
+            }
+        }
+        if (a.dw) {
+            const uint8_t* zl = smem + turned + wn * (NT * 32);
+            const uint8_t* xl = smem + L::X + turned + wk * (KT * 32);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                bf16x8 x[KT / 2];
+#pragma unroll
+                for (int i = 0; i < KT / 2; ++i) x[i] = read_turned(xl + (half * (KT / 2) + i) * 32, 4 * PITCH);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) {
+                        const bf16x8 z = read_turned(zl + k * L::PLANE + j * 32, 4 * PITCH);
+#pragma unroll
+                        for (int i = 0; i < KT / 2; ++i)
+                            acc[half * (KT / 2) + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], z, acc[half * (KT / 2) + i][j], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+        }
+    }
+
+    if (a.dw) {     // this workgroup's sums: lane holds four k of one n
+        float* s = a.slab + (int64_t)blockIdx.x * (C * C);
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                *reinterpret_cast<f32x4*>(s + ((wn * NT + j) * 16 + r) * C + (wk * KT + i) * 16 + q * 4) = acc[i][j];
+    }
+    if (a.colsum) {
+        __syncthreads();
+        float* s = reinterpret_cast<float*>(smem);      // [wave][256]
+        *reinterpret_cast<f32x4*>(s + wave * 256 + q * 64 + l16 * 4) = db;
+        __syncthreads();
+        if (tid < a.N) {
+            float v = 0.0f;
+            for (int i = 0; i < 8; ++i) v += s[i * 256 + tid];
+            a.colsum[(int64_t)blockIdx.x * a.N + tid] = v * a.factor;
+        }
+    }
+}
+
+// dW = factor * sum of the workgroups' parts, in their order: sixteen threads walk the parts of four neighbours, joined in order
+template <typename T, int C>
+__global__ __launch_bounds__(256) void mx_narrow_join_kernel(const float* __restrict__ slab, int groups, int N, int K, float factor,
+                                                            T* __restrict__ dw) {
+    __shared__ f32x4 part[16][16];
+    const int c = threadIdx.x & 15, w = threadIdx.x >> 4;
+    const int at = (blockIdx.x * 16 + c) * 4, n = at / C, k = at % C;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (n < N && k < K) {
+#pragma unroll 4
+        for (int g = w; g < groups; g += 16) v += *reinterpret_cast<const f32x4*>(slab + (int64_t)g * (C * C) + at);
+    }
+    part[w][c] = v;
+    __syncthreads();
+    if (w == 0 && n < N) {
+        f32x4 s = part[0][c];
+        for (int i = 1; i < 16; ++i) s += part[i][c];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (k + j < K) dw[(int64_t)n * K + k + j] = (T)(s[j] * factor);
+    }
+}
+
+template <typename T, int TERMS, int C, int SLOPE>
+int launch_bwd(const char* fn, NarrowBwd a, hipStream_t st) {
+    constexpr int lds = NarrowLds<T, TERMS, C>::BYTES;
+    static_assert(lds <= 160 * 1024 && 32 * C * 4 <= lds, "LDS");
+    int rc = nerf_set_lds(mx_narrow_bwd_kernel<T, TERMS, C, SLOPE>, lds);
+    if (rc) return rc;
+    a.whole = a.dx && (uintptr_t)a.dx % (4 * sizeof(T)) == 0 && a.lddx * sizeof(T) % (4 * sizeof(T)) == 0;
+    const int groups = narrow_groups(a.M);
+    mx_narrow_bwd_kernel<T, TERMS, C, SLOPE><<<(unsigned)groups, 512, lds, st>>>(a);
+    if ((rc = nerf_check_launch(fn)) || !a.dw) return rc;
+    mx_narrow_join_kernel<T, C><<<(unsigned)((a.N * C + 63) / 64), 256, 0, st>>>(a.slab, groups, a.N, a.K, a.factor, (T*)a.dw);
+    return nerf_check_launch(fn);
+}
+template <typename T, int TERMS, int SLOPE>
+int by_columns(const char* fn, const NarrowBwd& a, hipStream_t st) {
+    return narrow_columns(a.K, a.N) == 256 ? launch_bwd<T, TERMS, 256, SLOPE>(fn, a, st) : launch_bwd<T, TERMS, 128, SLOPE>(fn, a, st);
+}
+// terms without and with slopes (a ReLU's decisions need no more than none)
+template <typename T, int TERMS, int SMOOTH>
+int by_slope(const char* fn, const NarrowBwd& a, hipStream_t st) {
+    if (a.slope) return by_columns<T, SMOOTH, 1>(fn, a, st);
+    return a.mask ? by_columns<T, TERMS, 2>(fn, a, st) : by_columns<T, TERMS, 0>(fn, a, st);
+}
+
 }  // namespace
+
+int launch_narrow_bwd(const char* fn, const NarrowBwd& a, int dtype, hipStream_t st) {
+    if (dtype == NERF_F32) return by_slope<float, 3, 3>(fn, a, st);
+    if (dtype == NERF_F16) return by_slope<_Float16, 2, 2>(fn, a, st);
+    return by_slope<__bf16, 1, 2>(fn, a, st);
+}
 
 int launch_narrow_fwd(const char* fn, const NarrowFwd& a, int dtype, int act, hipStream_t st) {
     if (dtype == NERF_F32) return by_act<float>(fn, a, act, st);
