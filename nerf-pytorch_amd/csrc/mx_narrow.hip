@@ -152,7 +152,7 @@ int by_act(const char* fn, NarrowFwd a, int act, hipStream_t st) {
 
 // ------------------------------------------------------------------------------------------------------- backward
 // All three gradients in one pass over dy, the slopes and the packed x.  A workgroup of eight waves walks its 32-row pieces:
-//   * dy, slopes and codes of the next piece come straight into LDS while this one is multiplied;
+//   * dy and slopes of the next piece come straight into LDS while this one is multiplied, its codes into registers;
 //   * dz = dy * slope is split into bf16 terms, x is decoded, both as rows in LDS;
 //   * dx: the 32 rows times W, whose fragments every wave keeps in registers (an eighth of the columns each);
 //   * dW += dz^T x: each wave keeps a quarter by a half of the whole C x C result in accumulators to the end; the operands
@@ -168,9 +168,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base) {
 }
 __device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t b, uint8_t* dst, int voff) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)dst, 16, voff, 0, 0, 0);
-}
-__device__ __forceinline__ void to_lds4(__amdgpu_buffer_rsrc_t b, uint8_t* dst, int voff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)dst, 4, voff, 0, 0, 0);
 }
 // eight rows of a column: `at` is this lane's place for four of them, the other four lie `four` bytes on
 __device__ __forceinline__ bf16x8 read_turned(const uint8_t* at, int four) {
@@ -195,8 +192,8 @@ struct NarrowLds {
     static constexpr int PITCH = C * 2 + 32;                  // bytes of a row of bf16; 32 of padding spread rows over the banks
     static constexpr int PLANE = 32 * PITCH;
     static constexpr int X = TERMS * PLANE;                   // decoded x behind the terms of dz
-    static constexpr int DY = X + PLANE, SLOPE = DY + 32 * C * (int)sizeof(T), CODES = SLOPE + 32 * C * 4, SCALES = CODES + 32 * C / 2;
-    static constexpr int BYTES = SCALES + 256;
+    static constexpr int DY = X + PLANE, SLOPE = DY + 32 * C * (int)sizeof(T);
+    static constexpr int BYTES = SLOPE + 32 * C * 4;
 };
 
 // SLOPE: 0 none, 1 slopes, 2 decisions of a ReLU.
@@ -217,13 +214,11 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
     const int turned = (q * 8 + (r >> 2)) * PITCH + (r & 3) * 8;   // this lane's place in a 32 x 16 block read turned
 
     // codes of one row -> bf16 values in LDS
-    auto decode = [&](const uint8_t* codes, unsigned s, bool in) {
+    auto decode = [&](const unsigned (&c)[CODES / 8], unsigned s, bool in) {
         uint8_t* o = smem + L::X + row * PITCH + l16 * (CODES * 2);
 #pragma unroll
-        for (int i = 0; i < CODES / 8; ++i) {
-            const unsigned c = reinterpret_cast<const unsigned*>(codes)[i];
-            *reinterpret_cast<bf16x8*>(o + i * 16) = in ? decode8_bf16(c, s) : decode8_bf16(0u, 0u);
-        }
+        for (int i = 0; i < CODES / 8; ++i)
+            *reinterpret_cast<bf16x8*>(o + i * 16) = in ? decode8_bf16(c[i], s) : decode8_bf16(0u, 0u);
     };
 
     // this wave's columns of W, as the A operand of dx = dz W: 32 rows of W at a time through LDS
@@ -234,7 +229,10 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
             const int n = s * 32 + row, k = l16 * CODES;
             const bool in = n < a.N && k < steps * 128;
             const int64_t at = in ? (int64_t)n * (steps * 128) + k : 0;    // values from the first code
-            decode(a.wc + at / 2, a.ws[at / 32], in);
+            unsigned c[CODES / 8];
+#pragma unroll
+            for (int i = 0; i < CODES / 8; ++i) c[i] = reinterpret_cast<const unsigned*>(a.wc + at / 2)[i];
+            decode(c, a.ws[at / 32], in);
             __syncthreads();
 #pragma unroll
             for (int t = 0; t < XT; ++t) wf[t][s] = read_turned(smem + L::X + turned + (wave * XT + t) * 32, 4 * PITCH);
@@ -242,8 +240,10 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
         }
     }
 
-    constexpr int DYB = C * (int)sizeof(T), DYN = 32 * DYB / 1024, SLN = 32 * C * 4 / 1024, CON = 32 * C / 2 / 1024;
+    constexpr int DYB = C * (int)sizeof(T);
     [[maybe_unused]] uint16_t bits[CHUNKS];
+    unsigned codes[CODES / 8], scale;
+    // What wave w converts, rows 4w .. 4w + 3 of the piece, it also loads: no other wave is waited for.
     auto request = [&](int64_t piece) {
         // (hidden from the compiler, which would keep every lane's offsets in registers across the loop)
         int lane = threadIdx.x & 63, row = threadIdx.x >> 4, l16 = threadIdx.x & 15;
@@ -253,30 +253,25 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
         auto clamp = [&](int v) { return v < rows ? v : rows - 1; };
         const auto dy = rows_of((const T*)a.dy + m0 * a.lddy);
 #pragma unroll
-        for (int i = 0; i < (DYN + 7) / 8; ++i) {
-            const int p = i * 8 + wave;
-            if (DYN % 8 == 0 || p < DYN) {
-                const int byte = p * 1024 + lane * 16, c = byte % DYB;
-                to_lds16(dy, smem + L::DY + p * 1024, clamp(byte / DYB) * (int)a.lddy * (int)sizeof(T) + (c < a.N * (int)sizeof(T) ? c : 0));
-            }
+        for (int i = 0; i < 4 * DYB / 1024; ++i) {
+            const int c = lane * 16 % DYB, at = wave * 4 + (i * 1024 + lane * 16) / DYB;
+            to_lds16(dy, smem + L::DY + wave * (4 * DYB) + i * 1024,
+                     clamp(at) * (int)a.lddy * (int)sizeof(T) + (c < a.N * (int)sizeof(T) ? c : 0));
         }
         if constexpr (SLOPE == 1) {
             const auto sl = rows_of(a.slope + m0 * a.N);
 #pragma unroll
-            for (int i = 0; i < (SLN + 7) / 8; ++i) {
-                const int p = i * 8 + wave, byte = p * 1024 + lane * 16, c = byte % (C * 4);
-                to_lds16(sl, smem + L::SLOPE + p * 1024, clamp(byte / (C * 4)) * a.N * 4 + (c < a.N * 4 ? c : 0));
+            for (int i = 0; i < 4 * C * 4 / 1024; ++i) {
+                const int c = lane * 16 % (C * 4), at = wave * 4 + (i * 1024 + lane * 16) / (C * 4);
+                to_lds16(sl, smem + L::SLOPE + wave * (16 * C) + i * 1024, clamp(at) * a.N * 4 + (c < a.N * 4 ? c : 0));
             }
         }
-        if (a.dw && wave < CON + 1) {
-            if (wave < CON) {
-                const int byte = wave * 1024 + lane * 16, c = byte % (C / 2);
-                to_lds16(rows_of(a.xc + m0 * (steps * 64)), smem + L::CODES + wave * 1024,
-                         clamp(byte / (C / 2)) * (steps * 64) + (c < steps * 64 ? c : 0));
-            } else {
-                const int byte = lane * 4, c = byte % (C / 32);      // C = 128: the upper lanes repeat rows, behind what is read
-                to_lds4(rows_of(a.xs + m0 * (steps * 4)), smem + L::SCALES, clamp(byte / (C / 32) % 32) * (steps * 4) + (c < steps * 4 ? c : 0));
-            }
+        if (a.dw) {
+            const int k = l16 * CODES < steps * 128 ? l16 * CODES : 0;
+            const int64_t at = (m0 + clamp(row)) * (steps * 128) + k;    // values from the first code
+#pragma unroll
+            for (int i = 0; i < CODES / 8; ++i) codes[i] = reinterpret_cast<const unsigned*>(a.xc + at / 2)[i];
+            scale = a.xs[at / 32];
         }
         if constexpr (SLOPE == 2) {
             const int words = (a.N + 15) / 16;
@@ -325,8 +320,27 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
                 for (int j = 0; j < 4; ++j) v[j] = bits[i] >> (4 * (l16 & 3) + j) & 1 ? v[j] : 0.0f;
             }
             __bf16 t[4][TERMS];
+            unsigned top = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) split_terms<TERMS>(v[j], t[j]);
+            for (int j = 0; j < 4; ++j) {
+                const float x = v[j];
+                const unsigned b = __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
+                top = b > top ? b : top;
+            }
+            if (__any(top >= 0x7f7f8000u)) {    // not finite, or infinite as bf16: the careful way
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split_terms<TERMS>(v[j], t[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float x = v[j];
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) {
+                        t[j][k] = (__bf16)x;
+                        x -= (float)t[j][k];
+                    }
+                }
+            }
             dz[i] = v;
 #pragma unroll
             for (int k = 0; k < TERMS; ++k)
@@ -335,12 +349,11 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) db[j] += rows_sum(dz[0][j], dz[1][j], dz[2][j], dz[3][j]);
-        if (a.dw) {
-            const int k = l16 * CODES;
-            decode(smem + L::CODES + row * (C / 2) + k / 2, smem[L::SCALES + row * (C / 32) + k / 32], in_row && k < steps * 128);
-        }
-        __syncthreads();
+        if (a.dw) decode(codes, scale, in_row && l16 * CODES < steps * 128);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read its rows
         if (piece + gridDim.x < pieces) request(piece + gridDim.x);
+        __builtin_amdgcn_s_barrier();                           // (not __syncthreads(): the requests stay under way)
+        asm volatile("" ::: "memory");
 
         if (a.dx) {
 #pragma unroll
