@@ -28,6 +28,7 @@ __device__ __forceinline__ void unrolled(F&& f) {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -127,6 +128,16 @@ __device__ __forceinline__ unsigned quad_or(unsigned m) {
     m |= (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true);
     return m | (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true);
 }
+
+// The transposing LDS read (ds_read_b64_tr_b16): sixteen lanes name four rows of sixteen 16-bit values (lane i: row i / 4,
+// values 4 (i % 4) ..), lane j gets value j of the four rows.
+// eight rows of a column: `at` is this lane's place for four of them, the other four lie `four` bytes on
+__device__ __forceinline__ bf16x8 read_turned(const uint8_t* at, int four) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + four));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 
 // what every entry point checks of its sizes: 32-bit offsets inside a tile of 256 rows, int row counts of weights
 static inline bool sizes_ok(int64_t rows, int64_t K) { return rows >= 0 && K >= 1 && K <= (1 << 22) && rows <= (1ll << 40) / K; }

@@ -535,7 +535,8 @@ __global__ __launch_bounds__(256) void mx_finish_kernel(Finish f, int64_t M, int
 // ---------------------------------------------------------------------------------------------- gradients: operands
 // dz = dy * (d y / d z), split into bf16 terms: rows [term][M][Np] for the data gradient and, turned, [term][N][Mp] for
 // the weight gradient (either may be NULL); Np, Mp: rounded up to 64, zeros behind the end.  colsum: partial column sums
-// of dz [grid.y][N], or NULL.  Tiles of 64 x 64 through LDS, `deep` of them one under the other per workgroup.
+// of dz [grid.y][N], or NULL.  Tiles of 64 x 64, `deep` of them one under the other per workgroup; the terms go through LDS
+// as rows and are read out turned.
 struct DzArgs {
     const void* dy;
     int64_t lddy;
@@ -553,21 +554,25 @@ struct DzArgs {
 
 template <typename T, int TERMS>
 __global__ __launch_bounds__(256) void mx_dz_kernel(DzArgs a) {
-    __shared__ float tile[64 * 65];
-    const int tid = threadIdx.x;
+    constexpr int PITCH = 160, PLANE = 64 * PITCH;          // bytes: 64 bf16 and 32 of padding
+    __shared__ __attribute__((aligned(16))) uint8_t tile[TERMS * PLANE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n0 = blockIdx.x * 64;
-    const int lr = tid >> 2, lc = (tid & 3) * 16;     // reading: a row, sixteen columns
-    float csum = 0.0f;
+    const int lr = tid >> 2, lc = (tid & 3) * 16;           // reading: a row, sixteen columns
+    const int r = lane & 15, q = lane >> 4;
+    const uint8_t* turned = tile + (q * 8 + (r >> 2)) * PITCH + wave * 32 + (r & 3) * 8;    // writing: sixteen columns a wave
+    float csum[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) csum[i] = 0.0f;
     for (int d = 0; d < a.deep; ++d) {
         const int64_t m0 = ((int64_t)blockIdx.y * a.deep + d) * 64;
         if (m0 >= a.Mp) break;
         const int64_t m = m0 + lr;
         float v[16];
         const T* p = (const T*)a.dy + m * a.lddy + n0 + lc;
-        const bool in_row = m < a.M;
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-        if (in_row) {
+        if (m < a.M) {
             if (n0 + lc + 16 <= a.N && ((uintptr_t)p % 16) == 0) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 8) {
@@ -602,52 +607,55 @@ __global__ __launch_bounds__(256) void mx_dz_kernel(DzArgs a) {
                 }
             }
         }
-        if (a.rows && m < a.M) {
-            __bf16 t[16][TERMS];
+        __bf16 t[16][TERMS];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) split_terms<TERMS>(v[i], t[i]);
+        for (int i = 0; i < 16; ++i) {
+            csum[i] += v[i];
+            split_terms<TERMS>(v[i], t[i]);
+        }
+        if (a.turned) __syncthreads();      // the previous tile has been read
 #pragma unroll
-            for (int k = 0; k < TERMS; ++k) {
+        for (int k = 0; k < TERMS; ++k) {
+            bf16x8 lo, hi;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { lo[i] = t[i][k]; hi[i] = t[8 + i][k]; }
+            if (a.rows && m < a.M) {
                 __bf16* o = a.rows + ((int64_t)k * a.M + m) * a.Np + n0 + lc;
-                bf16x8 lo, hi;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) { lo[i] = t[i][k]; hi[i] = t[8 + i][k]; }
                 *reinterpret_cast<bf16x8*>(o) = lo;
                 *reinterpret_cast<bf16x8*>(o + 8) = hi;
             }
+            if (a.turned) {
+                *reinterpret_cast<bf16x8*>(tile + k * PLANE + lr * PITCH + lc * 2) = lo;
+                *reinterpret_cast<bf16x8*>(tile + k * PLANE + lr * PITCH + lc * 2 + 16) = hi;
+            }
         }
-        if (a.turned || a.colsum) {
-            __syncthreads();    // the previous tile has been read
-#pragma unroll
-            for (int i = 0; i < 16; ++i) tile[lr * 65 + lc + i] = v[i];
+        if (a.turned) {
             __syncthreads();
-            const int nn = tid >> 2, mm = (tid & 3) * 16;   // writing: a column, sixteen rows
-            __bf16 t[16][TERMS];
-            float s = 0.0f;
+            const int n = n0 + wave * 16 + r;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = tile[(mm + i) * 65 + nn];
-                s += x;
-                split_terms<TERMS>(x, t[i]);
-            }
-            csum += s;
-            if (a.turned && n0 + nn < a.N) {
+            for (int k = 0; k < TERMS; ++k)
 #pragma unroll
-                for (int k = 0; k < TERMS; ++k) {
-                    __bf16* o = a.turned + ((int64_t)k * a.N + n0 + nn) * a.Mp + m0 + mm;
-                    bf16x8 lo, hi;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) { lo[i] = t[i][k]; hi[i] = t[8 + i][k]; }
-                    *reinterpret_cast<bf16x8*>(o) = lo;
-                    *reinterpret_cast<bf16x8*>(o + 8) = hi;
+                for (int h = 0; h < 2; ++h) {
+                    const bf16x8 c = read_turned(turned + k * PLANE + h * (32 * PITCH), 4 * PITCH);
+                    if (n < a.N) *reinterpret_cast<bf16x8*>(a.turned + ((int64_t)k * a.N + n) * a.Mp + m0 + h * 32 + q * 8) = c;
                 }
-            }
         }
     }
-    if (a.colsum) {     // the quad's four partial sums, always in the same order
-        csum += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, csum), 0xB1, 0xf, 0xf, true));
-        csum += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, csum), 0x4E, 0xf, 0xf, true));
-        if ((tid & 3) == 0 && n0 + (tid >> 2) < a.N) a.colsum[(int64_t)blockIdx.y * a.N + n0 + (tid >> 2)] = csum * a.factor;
+    if (a.colsum) {     // the sixteen rows of a wave, then the four waves, always in the same order
+        float* part = reinterpret_cast<float*>(tile);       // [wave][64]
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s = csum[i];
+            s += __shfl_xor(s, 4);
+            s += __shfl_xor(s, 8);
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if (lane < 4) part[wave * 64 + lane * 16 + i] = s;
+        }
+        __syncthreads();
+        if (tid < 64 && n0 + tid < a.N)
+            a.colsum[(int64_t)blockIdx.y * a.N + n0 + tid] = (((part[tid] + part[64 + tid]) + part[128 + tid]) + part[192 + tid]) * a.factor;
     }
 }
 
@@ -671,8 +679,10 @@ __global__ __launch_bounds__(256) void mx_colsum_kernel(const float* __restrict_
 // packed rows [rows][K] -> turned bf16 values [K][rows_p], zeros behind the last row.  Tiles of 64 rows x 128 values.
 __global__ __launch_bounds__(256) void mx_turn_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
                                                      int64_t K, int64_t rows_p, __bf16* __restrict__ out) {
-    __shared__ __bf16 tile[64 * 130];
-    const int tid = threadIdx.x;
+    constexpr int PITCH = 288;                              // bytes: 128 bf16 and 32 of padding
+    __shared__ __attribute__((aligned(16))) uint8_t tile[64 * PITCH];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 15, q = lane >> 4;
     const int64_t m0 = (int64_t)blockIdx.y * 64, k0 = (int64_t)blockIdx.x * 128;
     const int64_t m = m0 + (tid >> 2);
     u32x4 c = {0u, 0u, 0u, 0u};
@@ -683,24 +693,18 @@ __global__ __launch_bounds__(256) void mx_turn_kernel(const uint8_t* __restrict_
         s = scales[block];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bf16x8 v = decode8_bf16(c[i], s);
-        unsigned* o = reinterpret_cast<unsigned*>(tile + (tid >> 2) * 130 + (tid & 3) * 32 + i * 8);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = __builtin_bit_cast(unsigned, bf16x2{v[2 * j], v[2 * j + 1]});
-    }
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<bf16x8*>(tile + (tid >> 2) * PITCH + (tid & 3) * 64 + i * 16) = decode8_bf16(c[i], s);
     __syncthreads();
-    const int kk = tid >> 1, mm = (tid & 1) * 32;
-    if (k0 + kk < K) {
-        __bf16* o = out + (k0 + kk) * rows_p + m0 + mm;
+    const uint8_t* turned = tile + (q * 8 + (r >> 2)) * PITCH + wave * 64 + (r & 3) * 8;    // 32 values of the row a wave
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            bf16x8 v;
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = tile[(mm + i + j) * 130 + kk];
-            *reinterpret_cast<bf16x8*>(o + i) = v;
+        for (int h = 0; h < 2; ++h) {
+            const bf16x8 v = read_turned(turned + j * 32 + h * (32 * PITCH), 4 * PITCH);
+            const int64_t k = k0 + wave * 32 + j * 16 + r;
+            if (k < K) *reinterpret_cast<bf16x8*>(out + k * rows_p + m0 + h * 32 + q * 8) = v;
         }
-    }
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -866,11 +870,14 @@ template <typename T>
 int backward(const char* fn, const BwdLayout& l, DzArgs dz, const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes,
              const uint8_t* wscales, int64_t M, int64_t K, int64_t N, uint8_t* ws, void* dx, int64_t lddx, void* dw, void* db,
              hipStream_t st) {
-    dz.rows = dx ? (__bf16*)(ws + l.rows) : nullptr;
+    // bf16 without a slope, in rows that the product can take: dy is its own one term
+    const bool direct = __is_same(T, __bf16) && !dz.slope && !dz.mask && N % 64 == 0 && (uintptr_t)dz.dy % 16 == 0 && dz.lddy % 8 == 0 &&
+                        dz.lddy < (1 << 22);
+    dz.rows = dx && !direct ? (__bf16*)(ws + l.rows) : nullptr;
     dz.turned = dw ? (__bf16*)(ws + l.turned) : nullptr;
     dz.colsum = db ? (float*)(ws + l.part) : nullptr;
-    int rc = launch_dz<T>(fn, dz, l.terms, st);
-    if (rc) return rc;
+    int rc = NERF_OK;
+    if ((dz.rows || dz.turned || dz.colsum) && (rc = launch_dz<T>(fn, dz, l.terms, st))) return rc;
     constexpr int dtype = sizeof(T) == 4 ? NERF_F32 : __is_same(T, __bf16) ? NERF_BF16 : NERF_F16;
     if (db && (rc = launch_colsum(fn, dz.colsum, (int)l.parts, (int)N, dtype, db, st))) return rc;
     if (dx) {   // dx[m][k] = sum over n of dz[m][n] W[n][k]
@@ -879,7 +886,7 @@ int backward(const char* fn, const BwdLayout& l, DzArgs dz, const uint8_t* xcode
         if ((rc = nerf_check_launch(fn))) return rc;
         GemmArgs a{};
         a.w = Operand{ws + l.wt, l.Np * 2, nullptr, 0, K, 0};
-        a.x = Operand{ws + l.rows, l.Np * 2, nullptr, 0, M, M * l.Np * 2};
+        a.x = direct ? Operand{(const uint8_t*)dz.dy, dz.lddy * 2, nullptr, 0, M, 0} : Operand{ws + l.rows, l.Np * 2, nullptr, 0, M, M * l.Np * 2};
         a.M = M;
         a.N = (int)K;
         a.steps = (int)(l.Np / 32);

@@ -161,21 +161,12 @@ int by_act(const char* fn, NarrowFwd a, int act, hipStream_t st) {
 //   * db: column sums in registers.
 // In the end every workgroup writes its dW and db sums, two small kernels add them in order.  262144 x 256 x 256 fp32 moves
 // 0.84 GB; ROUNDED.
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);   // addresses are clamped by hand
 }
 __device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t b, uint8_t* dst, int voff) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)dst, 16, voff, 0, 0, 0);
 }
-// eight rows of a column: `at` is this lane's place for four of them, the other four lie `four` bytes on
-__device__ __forceinline__ bf16x8 read_turned(const uint8_t* at, int four) {
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + four));
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
 // Sums over the four 16-lane rows of a wave of four values each: row i of the result holds value i's sum.
 __device__ __forceinline__ float rows_sum(float a, float b, float c, float d) {
     const auto add = [](unsigned x, unsigned y) { return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y); };
