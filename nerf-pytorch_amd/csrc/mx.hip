@@ -17,7 +17,7 @@ __device__ __forceinline__ int64_t row_of(int64_t i, int64_t total, int groups) 
 
 constexpr int UNROLL = 4;   // groups of eight values per thread, all loads of a thread in flight together
 
-template <typename T, bool VEC, bool FLAT>
+template <typename T, bool FLAT>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t total, int64_t K, int groups,
                                                          unsigned* __restrict__ codes, uint8_t* __restrict__ scales) {
     float v[UNROLL][8];
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
                 load8(x + i * 8, v[u]);
             } else {
                 const int64_t row = row_of(i, total, groups), k = (i - row * groups) * 8;
-                if (VEC && k + 8 <= K) load8(x + row * ldx + k, v[u]);
+                if (k + 8 <= K) load8(x + row * ldx + k, v[u]);
                 else load8_tail(x + row * ldx + k, K - k, v[u]);
             }
         } else {
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
     }
 }
 
-template <typename T, bool VEC, bool FLAT>
+template <typename T, bool FLAT>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                            int64_t total, int64_t K, int groups, T* __restrict__ out, int64_t ldo) {
     unsigned c[UNROLL], s[UNROLL];
@@ -74,16 +74,17 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned* __re
             if (k >= K) continue;
             p = out + row * ldo + k;
         }
-        if (FLAT || (VEC && k + 8 <= K)) {
+        if (FLAT || k + 8 <= K) {
             if constexpr (sizeof(T) == 4) {
                 float v[8];
                 decode8(c[u], s[u], v);
-                *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+                typedef typename Loose<float, 4>::type x4;
+                *reinterpret_cast<x4*>(p) = x4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<x4*>(p + 4) = x4{v[4], v[5], v[6], v[7]};
             } else if constexpr (__is_same(T, __bf16)) {
-                *reinterpret_cast<bf16x8*>(p) = decode8_bf16(c[u], s[u]);
+                *reinterpret_cast<typename Loose<T, 8>::type*>(p) = decode8_bf16(c[u], s[u]);
             } else {
-                *reinterpret_cast<f16x8*>(p) = decode8_f16(c[u], s[u]);
+                *reinterpret_cast<typename Loose<T, 8>::type*>(p) = decode8_f16(c[u], s[u]);
             }
         } else {
             const int n = K - k < 8 ? (int)(K - k) : 8;
@@ -113,13 +114,10 @@ void quantize_as(const void* xv, int64_t ldx, int64_t M, int64_t K, uint8_t* cod
     const T* x = (const T*)xv;
     const int64_t groups = code_pitch(K) / 4, total = M * groups;
     const unsigned grid = (unsigned)ceil_div64(total, 256 * UNROLL);
-    const bool vec = (uintptr_t)x % 16 == 0 && (ldx * sizeof(T)) % 16 == 0;
-    if (vec && K % 128 == 0 && ldx == K)
-        mx_quantize_kernel<T, true, true><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
-    else if (vec)
-        mx_quantize_kernel<T, true, false><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
+    if (K % 128 == 0 && ldx == K)
+        mx_quantize_kernel<T, true><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
     else
-        mx_quantize_kernel<T, false, false><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
+        mx_quantize_kernel<T, false><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
 }
 
 template <typename T>
@@ -127,14 +125,11 @@ void dequantize_as(const uint8_t* codes, const uint8_t* scales, int64_t M, int64
     T* out = (T*)ov;
     const int64_t groups = code_pitch(K) / 4, total = M * groups;
     const unsigned grid = (unsigned)ceil_div64(total, 256 * UNROLL);
-    const bool vec = (uintptr_t)out % 16 == 0 && (ldo * sizeof(T)) % 16 == 0;
     const unsigned* c = (const unsigned*)codes;
-    if (vec && K % 128 == 0 && ldo == K)
-        mx_dequantize_kernel<T, true, true><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
-    else if (vec)
-        mx_dequantize_kernel<T, true, false><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
+    if (K % 128 == 0 && ldo == K)
+        mx_dequantize_kernel<T, true><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
     else
-        mx_dequantize_kernel<T, false, false><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
+        mx_dequantize_kernel<T, false><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
 }
 
 }  // namespace

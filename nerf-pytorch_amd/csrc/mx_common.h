@@ -38,11 +38,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-template <typename T> struct Vec;
-template <> struct Vec<float> { typedef f32x4 x4; };
-template <> struct Vec<__bf16> { typedef bf16x4 x4; };
-template <> struct Vec<_Float16> { typedef f16x4 x4; };
-
 // bytes of a packed row
 __host__ __device__ inline int64_t code_pitch(int64_t K) { return (K + 127) / 128 * 64; }
 __host__ __device__ inline int64_t scale_pitch(int64_t K) { return (K + 127) / 128 * 4; }
@@ -88,15 +83,20 @@ __device__ __forceinline__ f16x8 decode8_f16(unsigned c, unsigned s) {
     return f16x8{a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
 }
 
-// eight consecutive values of a row as floats; VEC: 16-byte loads (base and pitch aligned, all eight inside the row)
+// Vectors in global memory at the alignment of their elements: the hardware takes a vector access at any address, so rows
+// of odd length or pitch need no path of their own, only their tails do.
+template <typename T, int N> struct Loose { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
+
+// eight consecutive values of a row as floats
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+        typedef typename Loose<float, 4>::type x4;
+        const x4 a = *reinterpret_cast<const x4*>(p), b = *reinterpret_cast<const x4*>(p + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
     } else {
-        typedef T x8 __attribute__((ext_vector_type(8)));
+        typedef typename Loose<T, 8>::type x8;
         const x8 a = *reinterpret_cast<const x8*>(p);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (float)a[i];

@@ -60,7 +60,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void mx_few_kernel(FewArgs a)
             const int m = i / groups, k = (i - m * groups) * 8;
             const T* p = (const T*)a.x + m * a.ldx + k;
             float v[8];
-            if (a.vec && k + 8 <= a.K) load8(p, v);
+            if (k + 8 <= a.K) load8(p, v);
             else load8_tail(p, (int64_t)a.K - k, v);
             const unsigned s = scale_byte(quad_max(amax8(v)));
             reinterpret_cast<unsigned*>(lc)[i] = encode8(v, s);
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void mx_few_kernel(FewArgs a)
         const int m = threadIdx.x >> 2, n = n0 + (threadIdx.x & 3) * 4;
         f32x4 v = part[threadIdx.x];
         for (int i = 1; i < waves; ++i) v += part[i * MT * 64 + threadIdx.x];
-        finish4<T, ACT, false>(a.f, v, m, n, a.N, m < a.M, load_bias<T>(a.f.bias, n, a.N), whole4<T>(a.f.out, a.f.ldo, n, a.N));
+        finish4<T, ACT, false>(a.f, v, m, n, a.N, m < a.M, load_bias<T>(a.f.bias, n, a.N));
     }
 }
 

@@ -39,16 +39,10 @@ __device__ __forceinline__ void activate(float z, const Finish& f, float& y, flo
     }
 }
 
-// Whether four neighbouring outputs of every row at column n can be stored as one vector (type of the output; fp32).
-template <typename T>
-__device__ __forceinline__ bool whole4(const void* base, int64_t pitch, int n, int N) {
-    return n + 4 <= N && ((uintptr_t)((const T*)base + n) | (uintptr_t)(pitch * sizeof(T))) % (4 * sizeof(T)) == 0;
-}
-
-// Four neighbouring outputs of one row (n .. n+3, those below N); whole: whole4() of the output.  The four lanes that hold
+// Four neighbouring outputs of one row (n .. n+3, those below N).  The four lanes that hold
 // sixteen neighbours of one row are a quad, or (ACROSS) sixteen lanes apart.
 template <typename T, int ACT, bool ACROSS>
-__device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, int n, int N, bool row_ok, const f32x4& bias, bool whole) {
+__device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, int n, int N, bool row_ok, const f32x4& bias) {
     f32x4 y, sl;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -74,11 +68,12 @@ __device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, i
     }
     if (!row_ok) return;
     T* o = (T*)f.out + m * f.ldo + n;
-    typename Vec<T>::x4 t;
+    typedef typename Loose<T, 4>::type x4;
+    x4 t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] = (T)y[i];
-    if (whole) {
-        *reinterpret_cast<typename Vec<T>::x4*>(o) = t;
+    if (n + 4 <= N) {
+        *reinterpret_cast<x4*>(o) = t;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -87,8 +82,8 @@ __device__ __forceinline__ void finish4(const Finish& f, f32x4 acc, int64_t m, i
     if constexpr (ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID) {
         if (f.slope) {
             float* s = f.slope + m * N + n;
-            if (whole4<float>(f.slope, N, n, N)) {
-                *reinterpret_cast<f32x4*>(s) = sl;
+            if (n + 4 <= N) {
+                *reinterpret_cast<typename Loose<float, 4>::type*>(s) = sl;
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -128,7 +123,6 @@ struct FewArgs {
     const uint8_t *wc, *ws;
     const void* x;
     int64_t ldx;
-    bool vec;               // 16-byte loads of x
     const uint8_t *xc, *xs;
     int M, K, N;
     int steps;              // of 128 values

@@ -73,18 +73,14 @@ template <int NI, int MI, typename T, int ACT>
 __device__ __forceinline__ void store_direct(const GemmArgs& a, const f32x4 (&acc)[NI][MI], int64_t m_first, int n_first) {
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     f32x4 bias[NI];
-    bool whole[NI];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        bias[i] = load_bias<T>(a.f.bias, n_first + i * 16 + q * 4, a.N);
-        whole[i] = whole4<T>(a.f.out, a.f.ldo, n_first + i * 16 + q * 4, a.N);
-    }
+    for (int i = 0; i < NI; ++i) bias[i] = load_bias<T>(a.f.bias, n_first + i * 16 + q * 4, a.N);
 #pragma unroll
     for (int j = 0; j < MI; ++j)
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int64_t m = m_first + j * 16 + r;
-            finish4<T, ACT, true>(a.f, acc[i][j], m, n_first + i * 16 + q * 4, a.N, m < a.M, bias[i], whole[i]);
+            finish4<T, ACT, true>(a.f, acc[i][j], m, n_first + i * 16 + q * 4, a.N, m < a.M, bias[i]);
             __builtin_amdgcn_sched_barrier(0);   // one group of registers at a time
         }
 }
@@ -98,7 +94,6 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int n = n_first + (lane % LPR) * 4;
     const f32x4 bias = a.f.slab ? f32x4{0.f, 0.f, 0.f, 0.f} : load_bias<T>(a.f.bias, n, a.N);
-    const bool whole = a.f.slab ? whole4<float>(a.f.slab, a.N, n, a.N) : whole4<T>(a.f.out, a.f.ldo, n, a.N);
     constexpr int U = ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID ? 2 : 8;   // rows in flight
 #pragma unroll
     for (int jj = 0; jj < MI; jj += 2) {
@@ -115,8 +110,8 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)
             if (a.f.slab) {
                 float* s = a.f.slab + ((int64_t)blockIdx.z * a.M + m) * a.N + n;
                 if (m < a.M) {
-                    if (whole) {
-                        *reinterpret_cast<f32x4*>(s) = v;
+                    if (n + 4 <= a.N) {
+                        *reinterpret_cast<typename Loose<float, 4>::type*>(s) = v;
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -124,7 +119,7 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)
                     }
                 }
             } else {
-                finish4<T, ACT, false>(a.f, v, m, n, a.N, m < a.M, bias, whole);
+                finish4<T, ACT, false>(a.f, v, m, n, a.N, m < a.M, bias);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -508,11 +503,15 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
         store_tile<NI, MI, T, ACT>(a, acc, reinterpret_cast<float*>(smem) + wave * store_tile_floats<NI>(), m0 + wm * 128, n0 + wn * 128);
 }
 
-// out = finish(sum of the slabs, in their order)
-template <typename T, int ACT>
+// out = finish(sum of the slabs): Z threads walk the slabs of four neighbours, joined in order.  A workgroup takes 1024 / Z
+// neighbours of one row's groups of sixteen.
+template <typename T, int ACT, int Z>
 __global__ __launch_bounds__(256) void mx_finish_kernel(Finish f, int64_t M, int N, int splits) {
+    constexpr int G = 256 / Z;
+    __shared__ f32x4 part[Z][G];
+    const int c = threadIdx.x % G, w = threadIdx.x / G;
     const int quads = (N + 15) / 16 * 4;    // groups of four, whole quads of lanes inside a row
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = (int64_t)blockIdx.x * G + c;
     const int64_t m = i / quads;
     const int n = (int)(i - m * quads) * 4;
     const bool ok = m < M;
@@ -520,16 +519,24 @@ __global__ __launch_bounds__(256) void mx_finish_kernel(Finish f, int64_t M, int
     if (ok && n < N) {
         const float* s = f.slab + m * N + n;
         const int64_t step = M * N;
-        if (N % 4 == 0) {
-            for (int z = 0; z < splits; ++z) v += *reinterpret_cast<const f32x4*>(s + z * step);
+        if (n + 4 <= N) {
+#pragma unroll 4
+            for (int z = w; z < splits; z += Z) v += *reinterpret_cast<const typename Loose<float, 4>::type*>(s + z * step);
         } else {
-            for (int z = 0; z < splits; ++z)
+            for (int z = w; z < splits; z += Z)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (n + j < N) v[j] += s[z * step + j];
         }
     }
-    finish4<T, ACT, false>(f, v, m, n, N, ok, load_bias<T>(f.bias, n, N), whole4<T>(f.out, f.ldo, n, N));
+    if constexpr (Z > 1) {
+        part[w][c] = v;
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int z = 1; z < Z; ++z) v += part[z][c];
+    }
+    finish4<T, ACT, false>(f, v, m, n, N, ok, load_bias<T>(f.bias, n, N));
 }
 
 // ---------------------------------------------------------------------------------------------- gradients: operands
@@ -573,7 +580,7 @@ __global__ __launch_bounds__(256) void mx_dz_kernel(DzArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0.0f;
         if (m < a.M) {
-            if (n0 + lc + 16 <= a.N && ((uintptr_t)p % 16) == 0) {
+            if (n0 + lc + 16 <= a.N) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 8) {
                     float t[8];
@@ -593,10 +600,10 @@ __global__ __launch_bounds__(256) void mx_dz_kernel(DzArgs a) {
             }
             if (a.slope) {
                 const float* s = a.slope + m * a.N + n0 + lc;
-                if (n0 + lc + 16 <= a.N && ((uintptr_t)s % 16) == 0) {
+                if (n0 + lc + 16 <= a.N) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
-                        const f32x4 t = *reinterpret_cast<const f32x4*>(s + i);
+                        const f32x4 t = *reinterpret_cast<const typename Loose<float, 4>::type*>(s + i);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) v[i + j] *= t[j];
                     }
@@ -766,7 +773,8 @@ int launch_gemm(const char* fn, GemmArgs a, const Plan& p, hipStream_t st) {
     int rc = p.large ? launch_gemm_large<KIND, T, ACT>(fn, a, p.splits, st) : launch_gemm_tile<KIND, 128, T, ACT>(fn, a, p.splits, st);
     if (rc || p.splits == 1) return rc;
     const int64_t items = a.M * ((a.N + 15) / 16 * 4);
-    mx_finish_kernel<T, ACT><<<(unsigned)ceil_div64(items, 256), 256, 0, st>>>(a.f, a.M, a.N, p.splits);
+    if (p.splits >= 8) mx_finish_kernel<T, ACT, 16><<<(unsigned)ceil_div64(items, 16), 256, 0, st>>>(a.f, a.M, a.N, p.splits);
+    else mx_finish_kernel<T, ACT, 1><<<(unsigned)ceil_div64(items, 256), 256, 0, st>>>(a.f, a.M, a.N, p.splits);
     return nerf_check_launch(fn);
 }
 
@@ -952,7 +960,7 @@ extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const u
     const Finish f{y, ldy, bias, (float)pre, (float)post, act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID ? slope : nullptr,
                    act == NERF_ACT_RELU ? mask : nullptr, (float*)(ws + l.slab)};
     if (l.narrow) {
-        const NarrowFwd a{x, ldx, M, (int)K, (int)N, wcodes, wscales, xcodes, xscales, false, false, f};
+        const NarrowFwd a{x, ldx, M, (int)K, (int)N, wcodes, wscales, xcodes, xscales, f};
         return launch_narrow_fwd(fn, a, dtype, act, st);
     }
     if (!l.fused) {
@@ -960,9 +968,7 @@ extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const u
         if (rc) return rc;
     }
     if (l.few) {
-        const int size = dtype == NERF_F32 ? 4 : 2;
-        const bool vec = (uintptr_t)x % 16 == 0 && ldx * size % 16 == 0;
-        const FewArgs a{wcodes, wscales, l.fused ? x : nullptr, ldx, vec, xc, xs, (int)M, (int)K, (int)N, (int)ceil_div64(K, 128), f};
+        const FewArgs a{wcodes, wscales, l.fused ? x : nullptr, ldx, xc, xs, (int)M, (int)K, (int)N, (int)ceil_div64(K, 128), f};
         return launch_few(fn, a, dtype, act, st);
     }
     GemmArgs a{};
@@ -1026,7 +1032,7 @@ extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const
     uint8_t* ws = (uint8_t*)workspace;
     if (l.narrow) {
         float* part = db ? (float*)(ws + l.part) : nullptr;
-        const NarrowBwd a{dy, lddy, dz.slope, dz.mask, dz.factor, xcodes, xscales, wcodes, wscales, M, (int)K, (int)N, dx, lddx, dw, (float*)ws, part, false};
+        const NarrowBwd a{dy, lddy, dz.slope, dz.mask, dz.factor, xcodes, xscales, wcodes, wscales, M, (int)K, (int)N, dx, lddx, dw, (float*)ws, part};
         int rc = launch_narrow_bwd(fn, a, dtype, st);
         return rc || !db ? rc : launch_colsum(fn, part, narrow_groups(M), (int)N, dtype, db, st);
     }

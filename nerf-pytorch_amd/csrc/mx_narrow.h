@@ -13,7 +13,6 @@ struct NarrowFwd {
     int K, N;
     const uint8_t *wc, *ws;
     uint8_t *xc, *xs;       // the rounded x for the backward pass, or NULL
-    bool vec, whole;        // four values of x, of y at a time (set by the launch)
     Finish f;
 };
 int launch_narrow_fwd(const char* fn, const NarrowFwd& a, int dtype, int act, hipStream_t st);
@@ -32,7 +31,6 @@ struct NarrowBwd {
     void* dw;
     float* slab;            // dw: [groups][C][C], C = 128 or 256
     float* colsum;          // [groups][N], or NULL
-    bool whole;             // four values of dx at a time (set by the launch)
 };
 // workgroups of the backward kernel: 32 rows at a time, four times at least
 static inline int narrow_groups(int64_t M) {

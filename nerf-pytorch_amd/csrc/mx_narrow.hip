@@ -57,10 +57,10 @@ __global__ __launch_bounds__(512, 4) void mx_narrow_fwd_kernel(NarrowFwd a) {
             v[i] = x4{};
             if (tile < tiles && m < a.M) {
                 const T* p = (const T*)a.x + m * a.ldx + k;
-                if (a.vec) {
-                    // vec: K is a multiple of four.  Non-temporal, x passes through once: 131 -> 121 us (ReLU); such stores of
+                if (k + 4 <= a.K) {
+                    // Non-temporal, x passes through once: 131 -> 121 us (ReLU); such stores of
                     // y, whose rows leave 64 bytes at a time, were slower (143 us).
-                    if (k < a.K) v[i] = __builtin_nontemporal_load(reinterpret_cast<const x4*>(p));
+                    v[i] = __builtin_nontemporal_load(reinterpret_cast<const typename Loose<T, 4>::type*>(p));
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(512, 4) void mx_narrow_fwd_kernel(NarrowFwd a) {
                 acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide8(w1), wide8(xf[1]), acc, 4, 4, 1, ws, 1, xs);
             }
             const f32x4 bias = *reinterpret_cast<const f32x4*>(bl + n);
-            finish4<T, ACT, true>(a.f, acc, m, n, a.N, ok, bias, a.whole && n + 4 <= a.N);
+            finish4<T, ACT, true>(a.f, acc, m, n, a.N, ok, bias);
         }
     }
 }
@@ -141,9 +141,7 @@ int by_steps(const char* fn, const NarrowFwd& a, hipStream_t st) {
     return a.K > 128 ? launch_fwd<T, ACT, 2>(fn, a, st) : launch_fwd<T, ACT, 1>(fn, a, st);
 }
 template <typename T>
-int by_act(const char* fn, NarrowFwd a, int act, hipStream_t st) {
-    a.vec = a.K % 4 == 0 && (uintptr_t)a.x % (4 * sizeof(T)) == 0 && a.ldx * sizeof(T) % (4 * sizeof(T)) == 0;
-    a.whole = (uintptr_t)a.f.out % (4 * sizeof(T)) == 0 && a.f.ldo * sizeof(T) % (4 * sizeof(T)) == 0;
+int by_act(const char* fn, const NarrowFwd& a, int act, hipStream_t st) {
     if (act == NERF_ACT_NONE) return by_steps<T, NERF_ACT_NONE>(fn, a, st);
     if (act == NERF_ACT_RELU) return by_steps<T, NERF_ACT_RELU>(fn, a, st);
     if (act == NERF_ACT_SIN) return by_steps<T, NERF_ACT_SIN>(fn, a, st);
@@ -371,8 +369,8 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
                         x4 v;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) v[j] = (T)(o[t][j] * a.factor);
-                        if (a.whole && k + 4 <= a.K) {
-                            *reinterpret_cast<x4*>(p) = v;
+                        if (k + 4 <= a.K) {
+                            *reinterpret_cast<typename Loose<T, 4>::type*>(p) = v;
                         } else {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
@@ -449,12 +447,11 @@ __global__ __launch_bounds__(256) void mx_narrow_join_kernel(const float* __rest
 }
 
 template <typename T, int TERMS, int C, int SLOPE>
-int launch_bwd(const char* fn, NarrowBwd a, hipStream_t st) {
+int launch_bwd(const char* fn, const NarrowBwd& a, hipStream_t st) {
     constexpr int lds = NarrowLds<T, TERMS, C>::BYTES;
     static_assert(lds <= 160 * 1024 && 32 * C * 4 <= lds, "LDS");
     int rc = nerf_set_lds(mx_narrow_bwd_kernel<T, TERMS, C, SLOPE>, lds);
     if (rc) return rc;
-    a.whole = a.dx && (uintptr_t)a.dx % (4 * sizeof(T)) == 0 && a.lddx * sizeof(T) % (4 * sizeof(T)) == 0;
     const int groups = narrow_groups(a.M);
     mx_narrow_bwd_kernel<T, TERMS, C, SLOPE><<<(unsigned)groups, 512, lds, st>>>(a);
     if ((rc = nerf_check_launch(fn)) || !a.dw) return rc;
