@@ -15,9 +15,10 @@ __device__ __forceinline__ int64_t row_of(int64_t i, int64_t total, int groups) 
     return total <= 0xffffffffll ? (int64_t)((unsigned)i / (unsigned)groups) : i / groups;
 }
 
-constexpr int UNROLL = 4;   // groups of eight values per thread, all loads of a thread in flight together
+// UNROLL: groups of eight values per thread, all loads of a thread in flight together: four, or one where that would leave
+// compute units without a workgroup (13 x 8000 fp16: SMALLQ).
 
-template <typename T, bool FLAT>
+template <typename T, bool FLAT, int UNROLL>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t total, int64_t K, int groups,
                                                          unsigned* __restrict__ codes, uint8_t* __restrict__ scales) {
     float v[UNROLL][8];
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
     }
 }
 
-template <typename T, bool FLAT>
+template <typename T, bool FLAT, int UNROLL>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                            int64_t total, int64_t K, int groups, T* __restrict__ out, int64_t ldo) {
     unsigned c[UNROLL], s[UNROLL];
@@ -113,23 +114,23 @@ template <typename T>
 void quantize_as(const void* xv, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, hipStream_t st) {
     const T* x = (const T*)xv;
     const int64_t groups = code_pitch(K) / 4, total = M * groups;
-    const unsigned grid = (unsigned)ceil_div64(total, 256 * UNROLL);
-    if (K % 128 == 0 && ldx == K)
-        mx_quantize_kernel<T, true><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
-    else
-        mx_quantize_kernel<T, false><<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales);
+    const bool flat = K % 128 == 0 && ldx == K, small = total <= 256 * 4 * 256;
+    const unsigned grid = (unsigned)ceil_div64(total, small ? 256 : 1024);
+    const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales); };
+    if (flat) small ? launch(mx_quantize_kernel<T, true, 1>) : launch(mx_quantize_kernel<T, true, 4>);
+    else small ? launch(mx_quantize_kernel<T, false, 1>) : launch(mx_quantize_kernel<T, false, 4>);
 }
 
 template <typename T>
 void dequantize_as(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* ov, int64_t ldo, hipStream_t st) {
     T* out = (T*)ov;
     const int64_t groups = code_pitch(K) / 4, total = M * groups;
-    const unsigned grid = (unsigned)ceil_div64(total, 256 * UNROLL);
+    const bool flat = K % 128 == 0 && ldo == K, small = total <= 256 * 4 * 256;
+    const unsigned grid = (unsigned)ceil_div64(total, small ? 256 : 1024);
     const unsigned* c = (const unsigned*)codes;
-    if (K % 128 == 0 && ldo == K)
-        mx_dequantize_kernel<T, true><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
-    else
-        mx_dequantize_kernel<T, false><<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo);
+    const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo); };
+    if (flat) small ? launch(mx_dequantize_kernel<T, true, 1>) : launch(mx_dequantize_kernel<T, true, 4>);
+    else small ? launch(mx_dequantize_kernel<T, false, 1>) : launch(mx_dequantize_kernel<T, false, 4>);
 }
 
 }  // namespace

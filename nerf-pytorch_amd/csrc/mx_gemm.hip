@@ -139,7 +139,7 @@ constexpr int store_tile_floats() { return 32 * (NI * 16 + 4); }
 // loads, barrier, [request the stage after it, read its first fragments | multiply the second half's].  One barrier a stage;
 // loads have a whole stage to arrive.
 template <int KIND, int TM, int TN, int WM, int WN, typename T, int ACT>
-__global__ __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 1) void mx_gemm_kernel(GemmArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 4) void mx_gemm_kernel(GemmArgs a) {
     constexpr int NW = WM * WN, MI = TM / WM / 16, NI = TN / WN / 16, R = TM + TN;
     constexpr int ROWS = R / NW;            // rows a wave stages: all of one operand
     constexpr int PIECES = ROWS / 8;        // 1 KiB requests: eight rows each
@@ -718,7 +718,7 @@ __global__ __launch_bounds__(256) void mx_turn_kernel(const uint8_t* __restrict_
 constexpr int kTargetGroups = 256;   // compute units
 
 struct Plan {
-    bool large;
+    int tile;
     int tiles_m, tiles_n, splits, per_split;
     size_t slab_floats;
 };
@@ -728,13 +728,13 @@ struct Plan {
 Plan plan_for(int64_t M, int64_t N, int64_t steps, int terms) {
     Plan p{};
     const int64_t total = (steps + 1) / 2 * terms;
-    p.large = ceil_div64(M, 256) * ceil_div64(N, 256) >= kTargetGroups * 3 / 4 && steps >= 4;   // (a window of scales is four steps)
-    const int t = p.large ? 256 : 128;
-    p.tiles_m = (int)ceil_div64(M, t);
-    p.tiles_n = (int)ceil_div64(N, t);
+    const auto tiles_of = [&](int64_t t) { return ceil_div64(M, t) * ceil_div64(N, t); };
+    p.tile = tiles_of(256) >= kTargetGroups * 3 / 4 && steps >= 4 ? 256 : tiles_of(128) >= kTargetGroups ? 128 : 64;   // (a window of scales is four steps)
+    p.tiles_m = (int)ceil_div64(M, p.tile);
+    p.tiles_n = (int)ceil_div64(N, p.tile);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     int64_t splits = 1;
-    if (!p.large && tiles < kTargetGroups) {
+    if (p.tile != 256 && tiles < kTargetGroups) {
         splits = kTargetGroups / tiles;
         const int64_t most = total / 4 < 1 ? 1 : total / 4;    // at least four stages a slice
         if (splits > most) splits = most;
@@ -770,7 +770,9 @@ int launch_gemm(const char* fn, GemmArgs a, const Plan& p, hipStream_t st) {
     a.tiles_n = p.tiles_n;
     a.per_split = p.per_split;
     if (p.splits == 1) a.f.slab = nullptr;
-    int rc = p.large ? launch_gemm_large<KIND, T, ACT>(fn, a, p.splits, st) : launch_gemm_tile<KIND, 128, T, ACT>(fn, a, p.splits, st);
+    int rc = p.tile == 256   ? launch_gemm_large<KIND, T, ACT>(fn, a, p.splits, st)
+             : p.tile == 128 ? launch_gemm_tile<KIND, 128, T, ACT>(fn, a, p.splits, st)
+                             : launch_gemm_tile<KIND, 64, T, ACT>(fn, a, p.splits, st);
     if (rc || p.splits == 1) return rc;
     const int64_t items = a.M * ((a.N + 15) / 16 * 4);
     if (p.splits >= 8) mx_finish_kernel<T, ACT, 16><<<(unsigned)ceil_div64(items, 16), 256, 0, st>>>(a.f, a.M, a.N, p.splits);
