@@ -570,52 +570,109 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int, dtype) -> t
     return out
 
 
+def _mx_bias(b: Optional[torch.Tensor], x: torch.Tensor, N: int) -> Optional[int]:
+    if b is None:
+        return None
+    if b.shape != (N,) or b.dtype != x.dtype or b.device != x.device:
+        raise ValueError(f"mx_linear: bias must be {x.dtype} [{N}] on {x.device}, got {b.dtype} {tuple(b.shape)} on {b.device}")
+    return _dev(b, "b", x.dtype)
+
+
 def mx_linear_fwd(x: torch.Tensor, wcodes: torch.Tensor, wscales: torch.Tensor, b: Optional[torch.Tensor], act: int, pre: float,
-                  post: float, train: bool = False):
-    """y [M,N] = post * f(pre * (Q(x) W^T + b)); with `train` also what the backward needs: (y, slope, mask, xcodes, xscales)."""
+                  post: float) -> torch.Tensor:
+    """y [M,N] = post * f(pre * (Q(x) W^T + b)), nothing kept."""
     ptr, dt, ld = _mx_rows(x, "x")
     M, K = x.shape
     N = wcodes.shape[0]
     pc, ps = _mx_packed(wcodes, wscales, K, x.device, "weight")
-    if b is not None and (b.shape != (N,) or b.dtype != x.dtype or b.device != x.device):
-        raise ValueError(f"mx_linear: bias must be {x.dtype} [{N}] on {x.device}, got {b.dtype} {tuple(b.shape)} on {b.device}")
-    slope = mask = xc = xs = None
+    pb = _mx_bias(b, x, N)
     y = x.new_empty((M, N))
-    if train:
-        if act in (ACT_SIN, ACT_SIGMOID):
-            slope = x.new_empty((M, N), dtype=torch.float32)
-        elif act == ACT_RELU:
-            mask = x.new_empty((M, (N + 15) // 16), dtype=torch.int16)
-        xc, xs = _mx_alloc(M, K, x)
-    nbytes = lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N, int(train))
+    nbytes = lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N, 0)
     ws = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     ev = timers.start("mx_linear_fwd", M)
-    rc = _mx_call(lib.nerf_mx_linear_fwd, x.get_device(), ptr, dt, ld, pc, ps, None if b is None else _dev(b, "b", x.dtype), M, K, N, act,
-                  pre, post, y.data_ptr(), N, None if slope is None else slope.data_ptr(), None if mask is None else mask.data_ptr(),
-                  None if xc is None else xc.data_ptr(), None if xs is None else xs.data_ptr(), None if ws is None else ws.data_ptr())
+    rc = _mx_call(lib.nerf_mx_linear_fwd, x.get_device(), ptr, dt, ld, pc, ps, pb, M, K, N, act, pre, post, y.data_ptr(), N, None, None,
+                  None, None, None if ws is None else ws.data_ptr())
     if rc:
         _check(rc, "nerf_mx_linear_fwd")
     timers.stop(ev)
-    return (y, slope, mask, xc, xs) if train else y
+    return y
 
 
-def mx_linear_bwd(dy: torch.Tensor, slope, mask, act: int, pre: float, post: float, xcodes, xscales, wcodes, wscales, K: int,
-                  need_dx: bool, need_dw: bool, need_db: bool):
-    """(dx [M,K], dW [N,K], db [N]) in the type of dy, None where not asked for."""
+class MXKept:
+    """What a training forward keeps for its backward, in one buffer: the packed x, the packed W where the call packed it,
+    slopes or ReLU decisions.  `packed` is a packed W that came from outside."""
+    __slots__ = ("buffer", "packed", "M", "K", "N", "act", "pre", "post", "xcodes", "xscales", "wcodes", "wscales", "extra")
+
+    def __init__(self, M, K, N, act, pre, post, packed):
+        self.M, self.K, self.N, self.act, self.pre, self.post, self.packed = M, K, N, act, pre, post, packed
+        blocks = (K + 127) // 128
+        at = 0
+
+        def take(n):
+            nonlocal at
+            start = at
+            at += -(-n // 256) * 256
+            return start
+        self.xcodes, self.xscales = take(64 * blocks * M), take(4 * blocks * M)
+        self.wcodes, self.wscales = (take(64 * blocks * N), take(4 * blocks * N)) if packed is None else (0, 0)
+        smooth = act == ACT_SIN or act == ACT_SIGMOID
+        self.extra = take(4 * M * N if smooth else 2 * M * ((N + 15) // 16)) if act != ACT_NONE else None
+        self.buffer = at      # its size, until the tensor takes the place
+
+
+def mx_linear_train(x: torch.Tensor, W: Optional[torch.Tensor], packed, b: Optional[torch.Tensor], act: int, pre: float, post: float):
+    """mx_linear_fwd for a backward pass: (y, MXKept).  W [N,K] float is packed here, or `packed` = (codes, scales) is taken."""
+    ptr, dt, ld = _mx_rows(x, "x")
+    M, K = x.shape
+    if packed is None:
+        wptr, wdt, wld = _mx_rows(W, "weight")
+        N = W.shape[0]
+    else:
+        N = packed[0].shape[0]
+        pc, ps = _mx_packed(*packed, K, x.device, "weight")
+    pb = _mx_bias(b, x, N)
+    kept = MXKept(M, K, N, act, pre, post, packed)
+    index = x.get_device()
+    y = x.new_empty((M, N))
+    buffer = kept.buffer = x.new_empty((kept.buffer,), dtype=torch.uint8)
+    base = buffer.data_ptr()
+    if packed is None:
+        pc, ps = base + kept.wcodes, base + kept.wscales
+        rc = _mx_call(lib.nerf_mx_quantize, index, wptr, wdt, wld, N, K, pc, ps)
+        if rc:
+            _check(rc, "nerf_mx_quantize")
+    extra = None if kept.extra is None else base + kept.extra
+    nbytes = lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N, 1)
+    ws = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    ev = timers.start("mx_linear_fwd", M)
+    rc = _mx_call(lib.nerf_mx_linear_fwd, index, ptr, dt, ld, pc, ps, pb, M, K, N, act, pre, post, y.data_ptr(), N,
+                  None if act == ACT_RELU else extra, extra if act == ACT_RELU else None, base + kept.xcodes, base + kept.xscales,
+                  None if ws is None else ws.data_ptr())
+    if rc:
+        _check(rc, "nerf_mx_linear_fwd")
+    timers.stop(ev)
+    return y, kept
+
+
+def mx_linear_bwd(dy: torch.Tensor, kept: MXKept, buffer: torch.Tensor, packed, need_dx: bool, need_dw: bool, need_db: bool):
+    """(dx [M,K], dW [N,K], db [N]) in the type of dy, None where not asked for; buffer, packed: kept's tensors."""
     ptr, dt, ld = _mx_rows(dy, "dy")
-    M, N = dy.shape
-    xp = _mx_packed(xcodes, xscales, K, dy.device, "x")
-    wp = _mx_packed(wcodes, wscales, K, dy.device, "weight")
-    if xcodes.shape[0] != M or wcodes.shape[0] != N:
-        raise ValueError(f"mx_linear_bwd: dy {tuple(dy.shape)} does not match x [{xcodes.shape[0]},{K}] and W [{wcodes.shape[0]},{K}]")
+    M, K, N, act = kept.M, kept.K, kept.N, kept.act
+    if dy.shape != (M, N):
+        raise ValueError(f"mx_linear_bwd: dy {tuple(dy.shape)} is not [{M},{N}]")
+    base = buffer.data_ptr()
+    if packed is None:
+        pc, ps = base + kept.wcodes, base + kept.wscales
+    else:
+        pc, ps = _mx_packed(*packed, K, dy.device, "weight")
+    extra = None if kept.extra is None else base + kept.extra
     dx = dy.new_empty((M, K)) if need_dx else None
     dw = dy.new_empty((N, K)) if need_dw else None
     db = dy.new_empty((N,)) if need_db else None
-    nbytes = lib.nerf_mx_linear_bwd_workspace_bytes(dt, act, M, K, N, need_dx, need_dw, need_db)
-    ws = dy.new_empty((nbytes,), dtype=torch.uint8)
+    ws = dy.new_empty((lib.nerf_mx_linear_bwd_workspace_bytes(dt, act, M, K, N, need_dx, need_dw, need_db),), dtype=torch.uint8)
     ev = timers.start("mx_linear_bwd", M)
-    rc = _mx_call(lib.nerf_mx_linear_bwd, dy.get_device(), ptr, dt, ld, None if slope is None else slope.data_ptr(),
-                  None if mask is None else mask.data_ptr(), act, pre, post, *xp, *wp, M, K, N, ws.data_ptr(),
+    rc = _mx_call(lib.nerf_mx_linear_bwd, dy.get_device(), ptr, dt, ld, None if act == ACT_RELU else extra, extra if act == ACT_RELU else None,
+                  act, kept.pre, kept.post, base + kept.xcodes, base + kept.xscales, pc, ps, M, K, N, ws.data_ptr(),
                   None if dx is None else dx.data_ptr(), K, None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr())
     if rc:
         _check(rc, "nerf_mx_linear_bwd")

@@ -87,7 +87,7 @@ def linear(x: Tensor, weight: Union[MXTensor, Tensor], bias: Optional[Tensor] = 
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (W is not None and W.requires_grad) or (bias is not None and bias.requires_grad)):
-        y = MXLinearFunction.apply(m, W, packed, bias, act, pre, post)
+        y = MXLinearFunction.apply(m, W, packed, bias, act, float(pre), float(post))
     else:
         if packed is None:
             packed = _hip.mx_quantize(W.detach())

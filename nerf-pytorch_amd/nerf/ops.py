@@ -321,25 +321,25 @@ class MXLinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, W, packed, b, act, pre, post):
-        wc, ws = packed if packed is not None else _hip.mx_quantize(W.detach())
-        y, slope, mask, xc, xs = _hip.mx_linear_fwd(x.detach(), wc, ws, b, act, pre, post, train=True)
-        ctx.cfg = (act, float(pre), float(post), x.shape[1])
-        ctx.save_for_backward(slope, mask, xc, xs, wc, ws)
+        y, kept = _hip.mx_linear_train(x, W, packed, b, act, pre, post)
+        ctx.save_for_backward(kept.buffer, *(packed or ()))
+        kept.buffer = kept.packed = None       # saved above: autograd watches over them
+        ctx.kept = kept
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        slope, mask, xc, xs, wc, ws = ctx.saved_tensors
-        act, pre, post, K = ctx.cfg
-        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
-        if dy.shape[0] == 0:    # no rows: sums over nothing
-            z = [dy.new_zeros((0, K)), dy.new_zeros((wc.shape[0], K)), dy.new_zeros((wc.shape[0],))]
+        buffer, *packed = ctx.saved_tensors
+        kept = ctx.kept
+        need = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3]
+        if kept.M == 0:    # no rows: sums over nothing
+            z = dy.new_zeros((0, kept.K)), dy.new_zeros((kept.N, kept.K)), dy.new_zeros((kept.N,))
             dx, dw, db = (t if n else None for t, n in zip(z, need))
         else:
-            if dy.stride(1) != 1 or dy.stride(0) < dy.shape[1]:    # expanded or transposed gradients (a sum's, for one)
-                dy = dy.contiguous()
-            dx, dw, db = _hip.mx_linear_bwd(dy, slope, mask, act, pre, post, xc, xs, wc, ws, K, *need)
+            if not dy.is_contiguous() and (dy.stride(1) != 1 or dy.stride(0) < dy.shape[1]):
+                dy = dy.contiguous()           # expanded or transposed (a sum's, for one)
+            dx, dw, db = _hip.mx_linear_bwd(dy, kept, buffer, packed or None, *need)
         return dx, dw, None, db, None, None, None
 
 

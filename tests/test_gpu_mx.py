@@ -473,9 +473,8 @@ def test_captured_and_replayed(M):
         return mx.linear(x, q, b, mx.ACT_RELU)
 
     def train():
-        wc, ws = _hip.mx_quantize(w)
-        y, slope, mask, xc, xs = _hip.mx_linear_fwd(x, wc, ws, b, mx.ACT_SIN, 1.0, 1.0, train=True)
-        return (y, *_hip.mx_linear_bwd(dy, slope, mask, mx.ACT_SIN, 1.0, 1.0, xc, xs, wc, ws, K, True, True, True))
+        y, kept = _hip.mx_linear_train(x, w, None, b, mx.ACT_SIN, 1.0, 1.0)
+        return (y, *_hip.mx_linear_bwd(dy, kept, kept.buffer, None, True, True, True))
 
     with torch.no_grad():
         serve(), train()
