@@ -275,7 +275,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 4) void mx_gemm_kerne
                                n0 + wn * (NI * 16));
 }
 
-// One matrix instruction of the large tile, accumulating IN PLACE in accumulator registers.  With the builtin the compiler
+// One matrix instruction of the large tile, accumulating IN PLACE.  With the builtin the compiler
 // takes the result for a new value: it moved the 256 accumulators of the large tile between register files and spilled.
 // What it no longer sees is the result's latency; settle_all() covers that where the sums are read.
 // BYTE: where in their registers the scales are.
@@ -284,12 +284,12 @@ __device__ __forceinline__ void mfma_in_place(f32x4& acc, const i32x4& w, const 
     static_assert(BYTE < 2, "");
     if constexpr (KIND == PACKED && BYTE == 0)
         asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
-                     : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+                     : "+v"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
     else if constexpr (KIND == PACKED)
         asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
-                     : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+                     : "+v"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
     else
-        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(w), "v"(x));
 }
 // The wait between the last matrix instructions and the first reads of their results (at most 16 passes of 4 cycles); every
 // accumulator passes through an empty statement behind it, so that no read moves in front.
@@ -299,29 +299,29 @@ __device__ __forceinline__ void settle_all(f32x4 (&acc)[NI][MI]) {
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < MI; ++j) asm volatile("" : "+a"(acc[i][j]));
+        for (int j = 0; j < MI; ++j) asm volatile("" : "+v"(acc[i][j]));
 }
 
-// The large tile: 256 x 256, four waves of 128 x 128 (one per SIMD: 256 accumulator registers, and per matrix instruction a
-// quarter less LDS traffic than eight waves of 128 x 64).  Stages as above, 128 bytes of each of the 512 rows, in two
-// buffers.  A stage's two halves are 64 matrix instructions each; during the first the second's fragments are read, then
-// -- everybody holds what it needs of this buffer -- comes the stage's one barrier, and during the second half the stage
-// after next is requested into the buffer and the next one's first fragments are read.  The barrier stands in front of
-// matrix instructions whose fragments are in registers, and a request has two halves (2 x 1024 cycles at the full rate) to
-// arrive.  The stream is written out by hand, two matrix instructions and what goes between them at a time; the requests
-// are spread over the whole half, because the four waves' 64 KiB take the vector cache all of it (64 bytes a cycle).
+// The large tile: 256 x 256, eight waves of 128 (m) x 64 (n), two on each SIMD: what one wave waits for to issue -- a request,
+// a fragment read -- the other's matrix instructions hide.  (Four waves of 128 x 128 read a third less LDS, but alone on their
+// SIMDs ran at FOURW.)  Stages as above, 128 bytes of each of the 512 rows, in two buffers.
+//
+// A stage's two halves are eight slots of four matrix instructions: slot j multiplies row fragment x[j] with the half's four
+// column fragments.  As soon as slot j is done, x[j] of the next half is read into its place, eight slots ahead; the column
+// fragments have two sets.  At the start of the second half everybody holds all it needs of the stage: there is the stage's
+// one barrier, behind it the stage after next is requested into the buffer, one piece a slot, and the reads go to the next
+// stage, which had a whole stage to arrive.
 //
 // PACKED: the order of the blocks inside a stage is free as long as both operands agree, and lane group q takes blocks
 // 2q and 2q + 1 of the eight in its two halves: their two scale bytes are neighbours, one 16-bit read per row and stage,
 // and the matrix instruction picks the byte.  Scales are requested for two stages at a time, 16 bytes a row (8-byte
 // requests of 512 rows cost the L2 as much as the codes did); the last window of a row is moved back to end with it.
 //
-// Rows of 64 bytes a stage in a ring of four (three halves for a request to arrive) were slower: requests of half a cache
-// line halve what the L2 delivers.
+// Rows of 64 bytes a stage in a ring of four were slower: requests of half a cache line halve what the L2 delivers.
 template <int KIND, typename T, int ACT>
-__global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
-    constexpr int TILE = 256, R = 512, NI = 8, MI = 8;
-    constexpr int PIECES = 16;              // requests of a wave per stage
+__global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
+    constexpr int TILE = 256, R = 512, NI = 4, MI = 8;
+    constexpr int PIECES = 8;               // requests of a wave per stage
     constexpr int STAGE = R * 128, SCALES = R * 16;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // two stages; PACKED: and two windows of scales
 
@@ -331,28 +331,24 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
     int n0;
     tile_of(a, (int)blockIdx.x, TILE, TILE, m0, n0);
 
-    // waves 0 and 1 stage the tile's 256 rows of W, 2 and 3 those of X; rows behind the last one repeat it (never stored)
-    const bool is_w = wave < 2;
+    // waves 0 to 3 stage the tile's 256 rows of W, 4 to 7 those of X; rows behind the last one repeat it (never stored)
+    const bool is_w = wave < 4;
     const Operand& op = is_w ? a.w : a.x;
-    const int64_t row0 = (is_w ? (int64_t)n0 : m0) + (wave & 1) * 128;
+    const int64_t row0 = (is_w ? (int64_t)n0 : m0) + (wave & 3) * 64;
     const int64_t left = op.rows - row0;
-    const int valid = left > 128 ? 128 : left < 1 ? 1 : (int)left;
+    const int valid = left > 64 ? 64 : left < 1 ? 1 : (int)left;
     const int64_t first = left < 1 ? op.rows - 1 : row0;
     const uint8_t* from = op.p + first * op.pitch;
     const int size = valid * (int)op.pitch, ssize = valid * (int)op.sc_pitch;
     const uint8_t* sfrom = KIND == PACKED ? op.sc + first * op.sc_pitch : nullptr;
     const int col = (lane & 7) ^ (lane >> 3);
-    int voff[PIECES], svoff[2];
+    int voff[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const int row = i * 8 + (lane >> 3);
         voff[i] = (row < valid ? row : valid - 1) * (int)op.pitch + col * 16;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = i * 64 + lane;
-        svoff[i] = (row < valid ? row : valid - 1) * (int)op.sc_pitch;
-    }
+    const int svoff = (lane < valid ? lane : valid - 1) * (int)op.sc_pitch;
     const int stages = (a.steps + 1) / 2;
     const bool odd = a.steps & 1;     // PACKED, one term: the last stage holds four blocks of eight
     const int D = stages * a.terms;   // the large tile does not split the reduction
@@ -364,14 +360,11 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
         int soff;
     };
     auto request = [&](int d) {
-        const Request rq{buffer_of(from, size), smem + (d & 1) * STAGE + wave * 16384, load_st * 128};
+        const Request rq{buffer_of(from, size), smem + (d & 1) * STAGE + wave * 8192, load_st * 128};
         if constexpr (KIND == PACKED) {
             if ((d & 1) == 0) {
                 const int window = d * 8, end = a.steps * 4 - 16;   // a.steps >= 4
-                const auto rows = buffer_of(sfrom, ssize);
-                uint8_t* dst = smem + 2 * STAGE + (d >> 1 & 1) * SCALES + wave * 2048;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) load_lds16(rows, dst + i * 1024, svoff[i], window < end ? window : end);
+                load_lds16(buffer_of(sfrom, ssize), smem + 2 * STAGE + (d >> 1 & 1) * SCALES + wave * 1024, svoff, window < end ? window : end);
             }
             if (odd && d == stages - 1) {   // read from the first four blocks instead, and not used (once per tile)
 #pragma unroll
@@ -386,31 +379,31 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
     };
     auto issue = [&](auto I, const Request& rq) { load_lds16(rq.rows, rq.dst + decltype(I)::value * 1024, voff[decltype(I)::value], rq.soff); };
 
-    const int wm = wave >> 1, wn = wave & 1;
+    const int wm = wave >> 2, wn = wave & 3;
     f32x4 acc[NI][MI];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < MI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    struct Frags {
-        i32x4 w[NI], x[MI];
-    } f0, f1;
+    i32x4 w0[NI], w1[NI], x[MI];
     struct Scales {
         int w[NI], x[MI];
     } scales, next_scales;   // both halves' of a stage
     const int piece0 = KIND == PACKED ? 2 * q : q, piece1 = KIND == PACKED ? 2 * q + 1 : 4 + q;
     const int place[2] = {r * 128 + ((piece0 ^ (r & 7)) * 16), r * 128 + ((piece1 ^ (r & 7)) * 16)};
     const int splace = 2 * STAGE + r * 16 + 2 * q;
-    auto read_one = [&](auto I, auto HALF, Frags& f, const uint8_t* stage, Scales& sc, int scale_at) {   // fragment I of 16: W and X by turns
-        constexpr int i = decltype(I)::value / 2, half = decltype(HALF)::value;
-        if constexpr (decltype(I)::value % 2 == 0) {
-            f.w[i] = *reinterpret_cast<const i32x4*>(stage + wn * 16384 + place[half] + i * 2048);
-            if constexpr (KIND == PACKED && half == 0)
-                sc.w[i] = *reinterpret_cast<const uint16_t*>(smem + splace + scale_at + wn * 2048 + i * 256);
-        } else {
-            f.x[i] = *reinterpret_cast<const i32x4*>(stage + 32768 + wm * 16384 + place[half] + i * 2048);
-            if constexpr (KIND == PACKED && half == 0)
-                sc.x[i] = *reinterpret_cast<const uint16_t*>(smem + splace + scale_at + 4096 + wm * 2048 + i * 256);
+    auto read_w = [&](auto I, auto HALF, i32x4 (&w)[NI], const uint8_t* stage) {
+        w[decltype(I)::value] = *reinterpret_cast<const i32x4*>(stage + wn * 8192 + place[decltype(HALF)::value] + decltype(I)::value * 2048);
+    };
+    auto read_x = [&](auto J, auto HALF, const uint8_t* stage) {
+        x[decltype(J)::value] =
+            *reinterpret_cast<const i32x4*>(stage + 32768 + wm * 16384 + place[decltype(HALF)::value] + decltype(J)::value * 2048);
+    };
+    auto read_scale = [&](auto I, Scales& sc, int scale_at) {   // I of 12: columns, then rows
+        constexpr int i = decltype(I)::value;
+        if constexpr (KIND == PACKED) {
+            if constexpr (i < NI) sc.w[i] = *reinterpret_cast<const uint16_t*>(smem + splace + scale_at + wn * 1024 + i * 256);
+            else sc.x[i - NI] = *reinterpret_cast<const uint16_t*>(smem + splace + scale_at + 4096 + wm * 2048 + (i - NI) * 256);
         }
     };
     // where the scales of stage d are: their window, and inside it (moved back by what the last window was)
@@ -418,17 +411,18 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
         const int window = (d >> 1) * 16, end = a.steps * 4 - 16;
         return (d >> 1 & 1) * SCALES + (d & 1) * 8 + (window > end ? window - end : 0);
     };
-    auto mfma = [&](auto U, auto HALF, const Frags& f) {
-        constexpr int j = decltype(U)::value / NI, i = decltype(U)::value % NI, half = decltype(HALF)::value;
-        mfma_in_place<KIND, half>(acc[i][j], f.w[i], f.x[j], KIND == PACKED ? scales.w[i] : 0, KIND == PACKED ? scales.x[j] : 0);
+    auto slot = [&](auto J, auto HALF, const i32x4 (&w)[NI]) {
+        constexpr int j = decltype(J)::value, half = decltype(HALF)::value;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            mfma_in_place<KIND, half>(acc[i][j], w[i], x[j], KIND == PACKED ? scales.w[i] : 0, KIND == PACKED ? scales.x[j] : 0);
     };
     // the last stage of an odd row: lane groups 2 and 3 multiply zeros (a branch around would put copies of the sums at its end)
-    auto blank = [&](Frags& f) {
+    auto blank = [&](i32x4 (&w)[NI]) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            f.w[i] = q < 2 ? f.w[i] : i32x4{0, 0, 0, 0};
-            f.x[i] = q < 2 ? f.x[i] : i32x4{0, 0, 0, 0};
-        }
+        for (int i = 0; i < NI; ++i) w[i] = q < 2 ? w[i] : i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < MI; ++j) x[j] = q < 2 ? x[j] : i32x4{0, 0, 0, 0};
     };
     auto publish = [&] {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -437,44 +431,47 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
     };
     constexpr std::integral_constant<int, 0> H0{};
     constexpr std::integral_constant<int, 1> H1{};
-    // Slot of fragment read k: two of every three slots up to the 24th; of request k: every other slot.
-    constexpr auto read_at = [](int u) { return u < 24 && u % 3 != 2 ? u / 3 * 2 + u % 3 : -1; };
-    // One stage: f0 holds its first half's fragments, and in the end the next stage's.
+    // One stage: x and w0 hold its first half's fragments, and in the end the next stage's.
     auto stage_body = [&](auto REQUEST, int d) {
         const uint8_t* here = smem + (d & 1) * STAGE;
         const uint8_t* next = smem + ((d & 1) ^ 1) * STAGE;
         if constexpr (!REQUEST)
             if (KIND == PACKED && odd && d == D - 1) {
-                blank(f0);
+                blank(w0);
 #pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    scales.w[i] = q < 2 ? scales.w[i] : 0;
-                    scales.x[i] = q < 2 ? scales.x[i] : 0;
-                }
+                for (int i = 0; i < NI; ++i) scales.w[i] = q < 2 ? scales.w[i] : 0;
+#pragma unroll
+                for (int j = 0; j < MI; ++j) scales.x[j] = q < 2 ? scales.x[j] : 0;
             }
         __builtin_amdgcn_sched_barrier(0);
-        unrolled<32>([&](auto U) {
-            constexpr int u = decltype(U)::value;
-            if constexpr (read_at(u) >= 0) read_one(std::integral_constant<int, read_at(u)>{}, H1, f1, here, scales, 0);
+        unrolled<MI>([&](auto J) {
+            constexpr int j = decltype(J)::value;
+            slot(J, H0, w0);
             __builtin_amdgcn_sched_barrier(0);
-            mfma(std::integral_constant<int, 2 * u>{}, H0, f0);
-            mfma(std::integral_constant<int, 2 * u + 1>{}, H0, f0);
+            read_x(J, H1, here);
+            if constexpr (j < NI) read_w(J, H1, w1, here);
             __builtin_amdgcn_sched_barrier(0);
         });
         publish();
         if constexpr (!REQUEST)
-            if (KIND == PACKED && odd && d == D - 1) blank(f1);
+            if (KIND == PACKED && odd && d == D - 1) blank(w1);
         Request rq;
         if constexpr (REQUEST) rq = request(d + 2);
         const int scale_at = scales_of(d + 1);
         __builtin_amdgcn_sched_barrier(0);
-        unrolled<32>([&](auto U) {
-            constexpr int u = decltype(U)::value;
-            if constexpr (REQUEST && u % 2 == 0) issue(std::integral_constant<int, u / 2>{}, rq);
-            if constexpr (read_at(u) >= 0) read_one(std::integral_constant<int, read_at(u)>{}, H0, f0, next, next_scales, scale_at);
+        unrolled<MI>([&](auto J) {
+            constexpr int j = decltype(J)::value;
+            if constexpr (REQUEST) issue(J, rq);
             __builtin_amdgcn_sched_barrier(0);
-            mfma(std::integral_constant<int, 2 * u>{}, H1, f1);
-            mfma(std::integral_constant<int, 2 * u + 1>{}, H1, f1);
+            slot(J, H1, w1);
+            __builtin_amdgcn_sched_barrier(0);
+            read_x(J, H0, next);
+            if constexpr (j < NI) {
+                read_w(J, H0, w0, next);
+                read_scale(std::integral_constant<int, 3 * j>{}, next_scales, scale_at);
+                read_scale(std::integral_constant<int, 3 * j + 1>{}, next_scales, scale_at);
+                read_scale(std::integral_constant<int, 3 * j + 2>{}, next_scales, scale_at);
+            }
             __builtin_amdgcn_sched_barrier(0);
         });
         scales = next_scales;
@@ -489,18 +486,20 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_large_kernel(GemmArgs a) {
         const Request rq = request(1);
         unrolled<PIECES>([&](auto I) { issue(I, rq); });
     }
-    unrolled<16>([&](auto I) { read_one(I, H0, f0, smem, scales, scales_of(0)); });
+    unrolled<NI>([&](auto I) { read_w(I, H0, w0, smem); });
+    unrolled<MI>([&](auto J) { read_x(J, H0, smem); });
+    unrolled<NI + MI>([&](auto I) { read_scale(I, scales, scales_of(0)); });
     int d = 0;   // (behind the last stage old contents are read, and not used)
     for (; d + 2 < D; ++d) stage_body(std::true_type{}, d);
     for (; d < D; ++d) stage_body(std::false_type{}, d);
     settle_all(acc);
     // nothing is under way; the barrier lets the last readers finish
-    static_assert(4 * store_tile_floats<NI>() * 4 <= 2 * STAGE, "the way out fits the stages");
+    static_assert(8 * store_tile_floats<NI>() * 4 <= 2 * STAGE, "the way out fits the stages");
     __syncthreads();
     if constexpr (ACT == NERF_ACT_NONE || ACT == NERF_ACT_RELU)
-        store_direct<NI, MI, T, ACT>(a, acc, m0 + wm * 128, n0 + wn * 128);
+        store_direct<NI, MI, T, ACT>(a, acc, m0 + wm * 128, n0 + wn * 64);
     else
-        store_tile<NI, MI, T, ACT>(a, acc, reinterpret_cast<float*>(smem) + wave * store_tile_floats<NI>(), m0 + wm * 128, n0 + wn * 128);
+        store_tile<NI, MI, T, ACT>(a, acc, reinterpret_cast<float*>(smem) + wave * store_tile_floats<NI>(), m0 + wm * 128, n0 + wn * 64);
 }
 
 // out = finish(sum of the slabs): Z threads walk the slabs of four neighbours, joined in order.  A workgroup takes 1024 / Z
@@ -760,7 +759,7 @@ int launch_gemm_large(const char* fn, const GemmArgs& a, int splits, hipStream_t
     constexpr int lds = 2 * (512 * 128 + (KIND == PACKED ? 512 * 16 : 0));
     int rc = nerf_set_lds(mx_gemm_large_kernel<KIND, T, ACT>, lds);
     if (rc) return rc;
-    mx_gemm_large_kernel<KIND, T, ACT><<<dim3((unsigned)(a.tiles_m * a.tiles_n), 1, (unsigned)splits), 256, lds, st>>>(a);
+    mx_gemm_large_kernel<KIND, T, ACT><<<dim3((unsigned)(a.tiles_m * a.tiles_n), 1, (unsigned)splits), 512, lds, st>>>(a);
     return nerf_check_launch(fn);
 }
 
