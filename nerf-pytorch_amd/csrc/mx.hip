@@ -10,103 +10,70 @@
 namespace mxk {
 namespace {
 
-// row of group i, in 32 bits wherever the count allows it (a 64-bit division is some hundred instructions)
-__device__ __forceinline__ int64_t row_of(int64_t i, int64_t total, int groups) {
-    return total <= 0xffffffffll ? (int64_t)((unsigned)i / (unsigned)groups) : i / groups;
-}
-
-// UNROLL: groups of eight values per thread, all loads of a thread in flight together: four, or one where that would leave
-// compute units without a workgroup (13 x 8000 fp16: SMALLQ).
-
-template <typename T, bool FLAT, int UNROLL>
+// One group of eight values per thread: two and four with all loads in flight together were slower, for small tensors (13 x
+// 8000 fp16: 2.6 against 3.4 us with four, compute units without a workgroup) as for large ones (reading 8192 x 8192 bf16: 61
+// against 68 us with four; rounding 262144 x 256 fp32: 50 against 52).
+template <typename T, bool FLAT>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t total, int64_t K, int groups,
                                                          unsigned* __restrict__ codes, uint8_t* __restrict__ scales) {
-    float v[UNROLL][8];
-    const int64_t base = (int64_t)blockIdx.x * (256 * UNROLL) + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const int64_t i = base + u * 256;
-        if (i < total) {
-            if constexpr (FLAT) {
-                load8(x + i * 8, v[u]);
-            } else {
-                const int64_t row = row_of(i, total, groups), k = (i - row * groups) * 8;
-                if (k + 8 <= K) load8(x + row * ldx + k, v[u]);
-                else load8_tail(x + row * ldx + k, K - k, v[u]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
-        }
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;   // below 2^32
+    if (i >= total) return;   // whole quads: a row is a multiple of sixteen groups
+    float v[8];
+    if constexpr (FLAT) {
+        load8(x + i * 8, v);
+    } else {
+        const int64_t row = (unsigned)i / (unsigned)groups, k = (i - row * groups) * 8;
+        if (k + 8 <= K) load8(x + row * ldx + k, v);
+        else load8_tail(x + row * ldx + k, K - k, v);
     }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const int64_t i = base + u * 256;
-        const unsigned s = scale_byte(quad_max(amax8(v[u])));
-        if (i < total) {
-            codes[i] = encode8(v[u], s);
-            if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)s;
-        }
-    }
+    const unsigned s = scale_byte(quad_max(amax8(v)));
+    codes[i] = encode8(v, s);
+    if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)s;
 }
 
-template <typename T, bool FLAT, int UNROLL>
+template <typename T, bool FLAT>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                            int64_t total, int64_t K, int groups, T* __restrict__ out, int64_t ldo) {
-    unsigned c[UNROLL], s[UNROLL];
-    const int64_t base = (int64_t)blockIdx.x * (256 * UNROLL) + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const int64_t i = base + u * 256;
-        c[u] = i < total ? codes[i] : 0u;
-        s[u] = i < total ? scales[i >> 2] : 0u;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const unsigned c = codes[i], s = scales[i >> 2];
+    int64_t k = 0;
+    T* p;
+    if constexpr (FLAT) {
+        p = out + i * 8;
+    } else {
+        const int64_t row = (unsigned)i / (unsigned)groups;
+        k = (i - row * groups) * 8;
+        if (k >= K) return;
+        p = out + row * ldo + k;
     }
+    T t[8];
+    if constexpr (sizeof(T) == 4) {
+        decode8(c, s, t);
+    } else if constexpr (__is_same(T, __bf16)) {
+        const bf16x8 v = decode8_bf16(c, s);
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const int64_t i = base + u * 256;
-        if (i >= total) continue;
-        int64_t row = 0, k = 0;
-        T* p;
-        if constexpr (FLAT) {
-            p = out + i * 8;
-        } else {
-            row = row_of(i, total, groups);
-            k = (i - row * groups) * 8;
-            if (k >= K) continue;
-            p = out + row * ldo + k;
+        for (int j = 0; j < 8; ++j) t[j] = v[j];
+    } else {
+        const f16x8 v = decode8_f16(c, s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = v[j];
+    }
+    if (FLAT || k + 8 <= K) {
+        typedef T t4 __attribute__((ext_vector_type(sizeof(T) == 4 ? 4 : 8)));
+        constexpr int L = sizeof(T) == 4 ? 4 : 8;
+#pragma unroll
+        for (int h = 0; h < 8 / L; ++h) {
+            t4 w;
+#pragma unroll
+            for (int j = 0; j < L; ++j) w[j] = t[h * L + j];
+            *reinterpret_cast<typename Loose<T, L>::type*>(p + h * L) = w;
         }
-        if (FLAT || k + 8 <= K) {
-            if constexpr (sizeof(T) == 4) {
-                float v[8];
-                decode8(c[u], s[u], v);
-                typedef typename Loose<float, 4>::type x4;
-                *reinterpret_cast<x4*>(p) = x4{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<x4*>(p + 4) = x4{v[4], v[5], v[6], v[7]};
-            } else if constexpr (__is_same(T, __bf16)) {
-                *reinterpret_cast<typename Loose<T, 8>::type*>(p) = decode8_bf16(c[u], s[u]);
-            } else {
-                *reinterpret_cast<typename Loose<T, 8>::type*>(p) = decode8_f16(c[u], s[u]);
-            }
-        } else {
-            const int n = K - k < 8 ? (int)(K - k) : 8;
-            T t[8];
-            if constexpr (sizeof(T) == 4) {
-                float v[8];
-                decode8(c[u], s[u], v);
-                for (int j = 0; j < 8; ++j) t[j] = v[j];
-            } else if constexpr (__is_same(T, __bf16)) {
-                const bf16x8 v = decode8_bf16(c[u], s[u]);
+    } else {
+        const int n = (int)(K - k);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) t[j] = v[j];
-            } else {
-                const f16x8 v = decode8_f16(c[u], s[u]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) t[j] = v[j];
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j < n) p[j] = t[j];
-        }
+        for (int j = 0; j < 8; ++j)
+            if (j < n) p[j] = t[j];
     }
 }
 
@@ -114,23 +81,23 @@ template <typename T>
 void quantize_as(const void* xv, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, hipStream_t st) {
     const T* x = (const T*)xv;
     const int64_t groups = code_pitch(K) / 4, total = M * groups;
-    const bool flat = K % 128 == 0 && ldx == K, small = total <= 256 * 4 * 256;
-    const unsigned grid = (unsigned)ceil_div64(total, small ? 256 : 1024);
+    const bool flat = K % 128 == 0 && ldx == K;
+    const unsigned grid = (unsigned)ceil_div64(total, 256);
     const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(x, ldx, total, K, (int)groups, (unsigned*)codes, scales); };
-    if (flat) small ? launch(mx_quantize_kernel<T, true, 1>) : launch(mx_quantize_kernel<T, true, 4>);
-    else small ? launch(mx_quantize_kernel<T, false, 1>) : launch(mx_quantize_kernel<T, false, 4>);
+    if (flat) launch(mx_quantize_kernel<T, true>);
+    else launch(mx_quantize_kernel<T, false>);
 }
 
 template <typename T>
 void dequantize_as(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* ov, int64_t ldo, hipStream_t st) {
     T* out = (T*)ov;
     const int64_t groups = code_pitch(K) / 4, total = M * groups;
-    const bool flat = K % 128 == 0 && ldo == K, small = total <= 256 * 4 * 256;
-    const unsigned grid = (unsigned)ceil_div64(total, small ? 256 : 1024);
+    const bool flat = K % 128 == 0 && ldo == K;
+    const unsigned grid = (unsigned)ceil_div64(total, 256);
     const unsigned* c = (const unsigned*)codes;
     const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(c, scales, total, K, (int)groups, out, ldo); };
-    if (flat) small ? launch(mx_dequantize_kernel<T, true, 1>) : launch(mx_dequantize_kernel<T, true, 4>);
-    else small ? launch(mx_dequantize_kernel<T, false, 1>) : launch(mx_dequantize_kernel<T, false, 4>);
+    if (flat) launch(mx_dequantize_kernel<T, true>);
+    else launch(mx_dequantize_kernel<T, false>);
 }
 
 }  // namespace

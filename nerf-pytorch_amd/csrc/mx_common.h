@@ -140,7 +140,10 @@ __device__ __forceinline__ bf16x8 read_turned(const uint8_t* at, int four) {
 
 
 // what every entry point checks of its sizes: 32-bit offsets inside a tile of 256 rows, int row counts of weights
-static inline bool sizes_ok(int64_t rows, int64_t K) { return rows >= 0 && K >= 1 && K <= (1 << 22) && rows <= (1ll << 40) / K; }
+// K up to 2^22; a thread for every eight values of the padded rows, less than 2^32 in a launch
+static inline bool sizes_ok(int64_t rows, int64_t K) {
+    return rows >= 0 && K >= 1 && K <= (1 << 22) && rows <= 0xffffff00ll / (code_pitch(K) / 4);
+}
 
 // launches shared between the files
 int launch_quantize(const char* fn, const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
