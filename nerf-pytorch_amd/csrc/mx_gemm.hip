@@ -67,8 +67,8 @@ __device__ __forceinline__ void tile_of(const GemmArgs& a, int t, int tm, int tn
 }
 
 // A wave's sums on their way out as they lie in the registers, four n of one m per lane: rows of 64 bytes (fp32) or 32 at a
-// time, joined in the L2.  For the light activations; half the instructions of the way through LDS, and with one wave per
-// SIMD those are what the end of a tile takes (4096 x 4096: 15 -> 10 us behind the products).
+// time, joined in the L2.  For the light activations: half the instructions of the way through LDS, and those are what the
+// end of a tile takes.
 template <int NI, int MI, typename T, int ACT>
 __device__ __forceinline__ void store_direct(const GemmArgs& a, const f32x4 (&acc)[NI][MI], int64_t m_first, int n_first) {
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 4) void mx_gemm_kerne
 }
 
 // One matrix instruction of the large tile, accumulating IN PLACE.  With the builtin the compiler
-// takes the result for a new value: it moved the 256 accumulators of the large tile between register files and spilled.
+// takes the result for a new value: it moved the large tile's accumulators between register files and spilled.
 // What it no longer sees is the result's latency; settle_all() covers that where the sums are read.
 // BYTE: where in their registers the scales are.
 template <int KIND, int BYTE>
@@ -304,7 +304,7 @@ __device__ __forceinline__ void settle_all(f32x4 (&acc)[NI][MI]) {
 
 // The large tile: 256 x 256, eight waves of 128 (m) x 64 (n), two on each SIMD: what one wave waits for to issue -- a request,
 // a fragment read -- the other's matrix instructions hide.  (Four waves of 128 x 128 read a third less LDS, but alone on their
-// SIMDs ran at FOURW.)  Stages as above, 128 bytes of each of the 512 rows, in two buffers.
+// SIMDs took 51 us where this takes 47, packed 4096 x 4096 x 4096, and 146 where it takes 141, 4096 x 8192 x 8192.)  Stages as above, 128 bytes of each of the 512 rows, in two buffers.
 //
 // A stage's two halves are eight slots of four matrix instructions: slot j multiplies row fragment x[j] with the half's four
 // column fragments.  As soon as slot j is done, x[j] of the next half is read into its place, eight slots ahead; the column
@@ -722,8 +722,13 @@ struct Plan {
     size_t slab_floats;
 };
 
-// Tile and split of an M x N product over `total` stages.
-// steps: 64-byte steps of a row.
+// Tile and split of an M x N product over rows of `steps` times 64 bytes.
+//
+// The largest tile that leaves no compute unit idle: a tile of 256 x 256 reads half of what 128 x 128 does for each product,
+// and a quarter of idle units is less than that (rounding and packed product in bf16, tiles of 128 against 256: 4096 x 4096 ->
+// 4096 70 : 54 us, 4096 x 8192 -> 8192 198 : 150, 3328 x 4096 -> 4096, 208 tiles, 60 : 47, 16384 x 1024 -> 1024 34 : 30).  Below
+// 256 tiles of 128 the work goes to tiles of 64 (1024^3 training in bf16 66 -> 53 us, 512 x 4096 -> 4096 32 -> 23.6 us, rows of
+// 319 -> 257 over 6000 in fp32 86 -> 74 us), and where those are too few the reduction is split.
 Plan plan_for(int64_t M, int64_t N, int64_t steps, int terms) {
     Plan p{};
     const int64_t total = (steps + 1) / 2 * terms;
@@ -802,8 +807,8 @@ struct FwdLayout {
 };
 FwdLayout fwd_layout(int64_t M, int64_t K, int64_t N, bool keeps_x) {
     FwdLayout l{};
-    l.few = M <= kFewRows;
-    l.narrow = M >= kNarrowRows && K <= kNarrow && N <= kNarrow;
+    l.few = few_rows(M, K, N);
+    l.narrow = M >= kNarrowRowsFwd && K <= kNarrow && N <= kNarrow;
     l.fused = (l.few && !keeps_x && few_fused(M, K)) || l.narrow;
     if (!l.few && !l.narrow) l.plan = plan_for(M, N, ceil_div64(K, 128), 1);
     if (!keeps_x && !l.fused) {
@@ -927,9 +932,11 @@ using namespace mxk;
 
 // M up to 2^30 rows, K and N up to 2^22: 32-bit offsets inside a tile, int tile counts
 static bool linear_sizes_ok(int64_t M, int64_t K, int64_t N) {
-    return M >= 0 && M <= (1 << 30) && K >= 1 && K <= (1 << 22) && N >= 1 && N <= (1 << 22) &&
-           ceil_div64(M, 128) * ceil_div64(N, 128) <= (1 << 30);
+    return M >= 0 && M <= (1 << 30) && sizes_ok(M, K) && N >= 1 && N <= (1 << 22) && sizes_ok(N, K) &&
+           ceil_div64(M, 128) * ceil_div64(N, 128) < (1 << 24);   // 2^32 threads in a launch
 }
+
+constexpr int64_t kTrainRows = 65535ll * 64;   // of a backward pass: grid.y; 32-bit offsets inside a turned tile
 
 extern "C" size_t nerf_mx_linear_fwd_workspace_bytes(int64_t M, int64_t K, int64_t N, int keeps_x) {
     return linear_sizes_ok(M, K, N) && M > 0 ? fwd_layout(M, K, N, keeps_x).bytes : 0;
@@ -943,6 +950,7 @@ extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const u
                  (long long)K, (long long)N, (long long)ldx, (long long)ldy);
     NERF_REQUIRE(dtype >= NERF_F32 && dtype <= NERF_F16, "%s: unknown type %d", fn, dtype);
     NERF_REQUIRE(act >= NERF_ACT_NONE && act <= NERF_ACT_SIGMOID, "%s: unknown activation %d", fn, act);
+    NERF_REQUIRE(!xcodes || M <= kTrainRows, "%s: more than 65535*64 rows kept for a backward pass", fn);
     if (M == 0) return NERF_OK;
     NERF_REQUIRE_PTR(x);
     NERF_REQUIRE_PTR(wcodes);
@@ -989,7 +997,7 @@ extern "C" size_t nerf_mx_linear_bwd_workspace_bytes(int dtype, int act, int64_t
                                                      int need_db) {
     if (!linear_sizes_ok(M, K, N) || M < 1 || dtype < NERF_F32 || dtype > NERF_F16) return 0;
     const size_t general = bwd_layout(dtype, act, M, K, N, need_dx, need_dw, need_db, false).bytes;
-    if (M < kNarrowRows || K > kNarrow || N > kNarrow) return general;
+    if (M < kNarrowRowsBwd || K > kNarrow || N > kNarrow) return general;
     const size_t narrow = bwd_layout(dtype, act, M, K, N, need_dx, need_dw, need_db, true).bytes;
     return narrow > general ? narrow : general;
 }
@@ -1003,7 +1011,7 @@ extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const
                  (long long)M, (long long)K, (long long)N);
     NERF_REQUIRE(dtype >= NERF_F32 && dtype <= NERF_F16, "%s: unknown type %d", fn, dtype);
     NERF_REQUIRE(act >= NERF_ACT_NONE && act <= NERF_ACT_SIGMOID, "%s: unknown activation %d", fn, act);
-    NERF_REQUIRE(M <= 65535ll * 64, "%s: more than 65535*64 rows per call", fn);   // grid.y; 32-bit offsets inside a turned tile
+    NERF_REQUIRE(M <= kTrainRows, "%s: more than 65535*64 rows per call", fn);
     if (!dx && !dw && !db) return NERF_OK;
     NERF_REQUIRE_PTR(dy);
     NERF_REQUIRE_PTR(workspace);
@@ -1016,7 +1024,7 @@ extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const
     const bool smooth = act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID;
     const int size = dtype == NERF_F32 ? 4 : 2;
     const BwdLayout l = bwd_layout(dtype, act, M, K, N, dx != nullptr, dw != nullptr, db != nullptr,
-                                   narrow_bwd_ok(dy, lddy, size, M, K, N, smooth ? slope : nullptr));
+                                   narrow_bwd_ok(dy, lddy, size, M, K, N, smooth && slope));
     DzArgs dz{};
     dz.dy = dy;
     dz.lddy = lddy;

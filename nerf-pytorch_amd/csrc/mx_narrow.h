@@ -5,7 +5,11 @@
 namespace mxk {
 
 constexpr int kNarrow = 256;            // inputs and outputs
-constexpr int64_t kNarrowRows = 4096;   // from here on the rows' bytes count, not the launches
+// Rows from which the fixed cost (weights read back, partial sums) is less than the bytes and launches that are saved.
+// Against the general way, us: forward 256 -> 256 relu fp32 with 8192 rows 11.3 : 8.2, 16384 13.6 : 14.4; sin fp32 with 12288
+// 17.7 : 11.6, 16384 18.5 : 18.7, 32768 23.1 : 23.6; 64 -> 64 with 32768 9.0 : 17.8.  Backward 256 -> 256 sin fp32 with 1024
+// 38.7 : 32.0, 4096 43.0 : 42.1, 8192 47.5 : 50.2, 65536 87 : 287; 64 -> 64 with 4096 19.9 : 24.9.
+constexpr int64_t kNarrowRowsFwd = 16384, kNarrowRowsBwd = 4096;
 
 struct NarrowFwd {
     const void* x;
@@ -40,7 +44,7 @@ static inline int narrow_groups(int64_t M) {
 static inline int narrow_columns(int64_t K, int64_t N) { return K > 128 || N > 128 ? 256 : 128; }
 // what the kernel's loads of whole 16-byte pieces ask of the layout
 static inline bool narrow_bwd_ok(const void* dy, int64_t lddy, int size, int64_t M, int64_t K, int64_t N, bool slope) {
-    return M >= kNarrowRows && K <= kNarrow && N <= kNarrow && (uintptr_t)dy % 16 == 0 && lddy * size % 16 == 0 && N * size % 16 == 0 &&
+    return M >= kNarrowRowsBwd && K <= kNarrow && N <= kNarrow && (uintptr_t)dy % 16 == 0 && lddy * size % 16 == 0 && N * size % 16 == 0 &&
            (!slope || N % 4 == 0) && lddy <= (1 << 20);
 }
 int launch_narrow_bwd(const char* fn, const NarrowBwd& a, int dtype, hipStream_t st);

@@ -158,7 +158,8 @@ int by_act(const char* fn, const NarrowFwd& a, int act, hipStream_t st) {
 //     column j of four rows);
 //   * db: column sums in registers.
 // In the end every workgroup writes its dW and db sums, two small kernels add them in order.  262144 x 256 x 256 fp32 moves
-// 0.84 GB; ROUNDED.
+// 0.84 GB in 296 us (sin; ReLU 0.60 GB in 255), and 12 + 7 us for the sums: bound by LDS, which every term of dz passes three times,
+// with the conversion between two products not overlapped.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);   // addresses are clamped by hand
 }

@@ -176,12 +176,31 @@ def test_linear_many_tiles(dtype, act, M, K, N):
     check_forward(mx.linear(x, w, b, mx.ACTIVATIONS[act]), x, w, b, act, 1.0, 1.0)
 
 
+FEW = [(16, 8192, 8192), (17, 8192, 8192), (26, 256, 300), (28, 256, 300), (64, 4096, 4096), (64, 4100, 4096), (65, 512, 512), (8, 40, 33000)]
+
+
+@pytest.mark.parametrize("M, K, N", FEW)
+def test_rows_of_a_batch_agree_with_single_rows(M, K, N):
+    """Both sides of the choice between the ways to multiply: every row as if it came alone, but for the order of its sums."""
+    from nerf import mx
+    x, q = randn(M, K, seed=1), mx.quantize(randn(N, K, seed=2, scale=K ** -0.5))
+    y = mx.linear(x, q)
+    assert torch.equal(y, mx.linear(x, q))
+    ax, aw = mx.dequantize(mx.quantize(x)).double(), mx.dequantize(q).double()
+    S = (ax.abs() @ aw.abs().t())
+    tol = 2 * (K * U * S + U * S) + 2.0 ** -23 * y.double().abs()
+    for m in {0, M // 2, M - 1}:
+        assert ((mx.linear(x[m:m + 1], q) - y[m:m + 1]).abs() <= tol[m:m + 1]).all()
+    assert ((y - ax @ aw.t()).abs() <= tol / 2).all()
+
+
+NARROW_FWD = [(16384, 256, 256), (16389, 100, 33), (16400, 31, 16), (17001, 255, 250), (16500, 132, 1), (20003, 128, 129), (16385, 1, 200)]
 NARROW = [(4096, 256, 256), (4111, 100, 33), (4097, 31, 16), (6001, 255, 250), (4500, 132, 1), (5003, 128, 129), (9000, 64, 64), (4099, 1, 200)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
-@pytest.mark.parametrize("M, K, N", NARROW)
+@pytest.mark.parametrize("M, K, N", NARROW_FWD)
 def test_linear_narrow(dtype, act, M, K, N):
     """Up to 256 inputs and outputs over many rows, ragged everywhere; then rows with a pitch and at an odd address."""
     from nerf import mx
@@ -240,17 +259,34 @@ def test_nan_stays_in_its_row_or_column(M):
         assert torch.equal(y[:, keep], clean[:, keep])
 
 
-def test_outputs_beside_the_rows_are_left_alone():
-    """The C entry with a pitch wider than the row: what lies between the rows keeps its contents."""
+@pytest.mark.parametrize("M, K, N", [(37, 160, 45), (300, 160, 45), (300, 1200, 45), (3400, 600, 3601), (16390, 160, 45)])
+@pytest.mark.parametrize("act", ["relu", "sin"])
+def test_outputs_beside_the_rows_are_left_alone(act, M, K, N):
+    """The C entries with a pitch wider than the row: what lies between the rows, and behind the last, keeps its contents."""
     from nerf import _hip, mx
-    M, K, N, ld = 37, 160, 45, 64
+    lib, ld, A = _hip.lib, N + 19, mx.ACTIVATIONS[act]
+    st = torch.cuda.current_stream().cuda_stream
     x, q = randn(M, K, seed=14), mx.quantize(randn(N, K, seed=15))
-    y = torch.full((M, ld), 7.0, device=DEV)
-    ws = torch.empty(_hip.lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N, 0), dtype=torch.uint8, device=DEV)
-    rc = _hip.lib.nerf_mx_linear_fwd(x.data_ptr(), 0, K, q.codes.data_ptr(), q.scales.data_ptr(), None, M, K, N, 0, 1.0, 1.0, y.data_ptr(), ld,
-                                     None, None, None, None, ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    y = torch.full((M + 3, ld), 7.0, device=DEV)
+    ws = torch.empty(lib.nerf_mx_linear_fwd_workspace_bytes(M, K, N, 0) + 16, dtype=torch.uint8, device=DEV)
+    rc = lib.nerf_mx_linear_fwd(x.data_ptr(), 0, K, q.codes.data_ptr(), q.scales.data_ptr(), None, M, K, N, A, 1.0, 1.0, y.data_ptr(), ld,
+                                None, None, None, None, ws.data_ptr(), st)
     assert rc == 0
-    assert torch.equal(y[:, :N], mx.linear(x, q)) and (y[:, N:] == 7.0).all()
+    assert torch.equal(y[:M, :N], mx.linear(x, q, None, A)) and (y[:, N:] == 7.0).all() and (y[M:] == 7.0).all()
+    want, kept = _hip.mx_linear_train(x, None, (q.codes, q.scales), None, A, 1.0, 1.0)
+    dy = randn(M, N, seed=16)
+    dx, dw, db = _hip.mx_linear_bwd(dy, kept, kept.buffer, (q.codes, q.scales), True, True, True)
+    base = kept.buffer.data_ptr()
+    wide, dw2, db2 = torch.full((M + 3, K + 5), 7.0, device=DEV), torch.full((N + 3, K), 7.0, device=DEV), torch.full((N + 9,), 7.0, device=DEV)
+    nbytes = lib.nerf_mx_linear_bwd_workspace_bytes(0, A, M, K, N, 1, 1, 1)
+    ws = torch.full((nbytes + 256,), 7, dtype=torch.uint8, device=DEV)
+    rc = lib.nerf_mx_linear_bwd(dy.data_ptr(), 0, N, base + kept.extra, base + kept.extra, A, 1.0, 1.0, base + kept.xcodes, base + kept.xscales,
+                                q.codes.data_ptr(), q.scales.data_ptr(), M, K, N, ws.data_ptr(), wide.data_ptr(), K + 5, dw2.data_ptr(),
+                                db2.data_ptr(), st)
+    assert rc == 0
+    assert torch.equal(wide[:M, :K], dx) and (wide[:, K:] == 7.0).all() and (wide[M:] == 7.0).all()
+    assert torch.equal(dw2[:N], dw) and (dw2[N:] == 7.0).all() and torch.equal(db2[:N], db) and (db2[N:] == 7.0).all()
+    assert (ws[nbytes:] == 7).all()
 
 
 # --------------------------------------------------------------------------------------------------------- gradients
@@ -324,7 +360,7 @@ def test_gradient_activations(dtype, act):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
-@pytest.mark.parametrize("M, K, N", NARROW)
+@pytest.mark.parametrize("M, K, N", NARROW + [(16390, 256, 256), (16387, 64, 40), (16500, 100, 129)])
 def test_gradients_narrow(dtype, act, M, K, N):
     x, w = randn(M, K, seed=31, dtype=dtype), randn(N, K, seed=32, dtype=dtype, scale=K ** -0.5)
     b = (torch.sign(randn(N, seed=33)) * 30).to(dtype) if act == "relu" else randn(N, seed=33, dtype=dtype)
@@ -459,12 +495,30 @@ def test_other_stream():
     assert torch.equal(q, mx.dequantize(mx.quantize(x)))
 
 
-@pytest.mark.parametrize("M", [1, 40, 700])
-def test_captured_and_replayed(M):
+def test_two_calls_at_once():
+    """The same layers forward and backward on two streams that run side by side, several times over."""
+    sets = [(randn(m, k, seed=1), randn(n, k, seed=2), randn(n, seed=3), randn(m, n, seed=4))
+            for m, k, n in ((20, 512, 300), (700, 256, 256), (17000, 256, 256), (3400, 300, 3601))]
+    want = [run_training(*s, "sin") for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(3):
+        for st, order in zip(streams, (sets, sets[::-1])):
+            with torch.cuda.stream(st):
+                got.append([run_training(*s, "sin") for s in order][::1 if order is sets else -1])
+    torch.cuda.synchronize()
+    for run in got:
+        for a, c in zip(run, want):
+            assert torch.equal(a[0], c[0]) and all(torch.equal(g, h) for g, h in zip(a[1], c[1]))
+
+
+@pytest.mark.parametrize("M, K, N", [(1, 512, 256), (40, 512, 256), (700, 512, 256), (5000, 128, 256), (16390, 256, 200), (3400, 520, 3601)])
+def test_captured_and_replayed(M, K, N):
     """Two captured graphs (a layer's product, and a product with its gradients), replayed alternately with new inputs
     and eager work between, against the eager results."""
     from nerf import _hip, mx
-    K, N = 512, 256
     w, b = randn(N, K, seed=81), randn(N, seed=82)
     q = mx.quantize(w)
     x, dy = randn(M, K, seed=83), randn(M, N, seed=84)

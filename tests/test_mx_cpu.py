@@ -90,7 +90,9 @@ def _fwd(**kw):
     (dict(ldx=31), -1, b"ldx=31"), (dict(ldy=7), -1, b"ldy=7"), (dict(dtype=5), -1, b"unknown type 5"),
     (dict(act=4), -1, b"unknown activation 4"), (dict(M=-1), -1, b"M=-1"), (dict(K=0), -1, b"K=0"), (dict(N=0), -1, b"N=0"),
     (dict(M=(1 << 30) + 1), -1, b"bad shape"), (dict(K=(1 << 22) + 1, ldx=1 << 23), -1, b"bad shape"),
-    (dict(M=1 << 30, N=1 << 22, ldy=1 << 22), -1, b"bad shape"),
+    (dict(M=1 << 30, N=1 << 22, ldy=1 << 22), -1, b"bad shape"), (dict(M=1 << 28), -1, b"bad shape"),
+    (dict(M=1 << 19, N=1 << 22, ldy=1 << 22), -1, b"bad shape"),       # 2^32 threads
+    (dict(xc=P, xs=P, M=65535 * 64 + 1), -1, b"kept for a backward pass"),
     (dict(xc=P), -1, b"go together"), (dict(wc=P + 4), -1, b"aligned"), (dict(work=P + 8), -1, b"aligned"),
     (dict(M=0, x=None, y=None, work=None), 0, b""),
 ])
