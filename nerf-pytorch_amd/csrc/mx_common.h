@@ -131,8 +131,9 @@ __device__ __forceinline__ unsigned quad_or(unsigned m) {
 
 // The transposing LDS read (ds_read_b64_tr_b16): sixteen lanes name four rows of sixteen 16-bit values (lane i: row i / 4,
 // values 4 (i % 4) ..), lane j gets value j of the four rows.
-// eight rows of a column: `at` is this lane's place for four of them, the other four lie `four` bytes on
-__device__ __forceinline__ bf16x8 read_turned(const uint8_t* at, int four) {
+// eight rows of a column: `at` is this lane's place for four of them, the other four lie `four` bytes on.  (Without __restrict__
+// the compiler takes the read for one of whatever is on its way from global memory to LDS, and waits for all of that.)
+__device__ __forceinline__ bf16x8 read_turned(const uint8_t* __restrict__ at, int four) {
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + four));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));

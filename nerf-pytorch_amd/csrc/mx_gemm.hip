@@ -831,7 +831,7 @@ BwdLayout bwd_layout(int dtype, int act, int64_t M, int64_t K, int64_t N, bool n
     BwdLayout l{};
     if (narrow) {
         l.narrow = true;
-        const int groups = narrow_groups(M), c = narrow_columns(K, N);
+        const int c = narrow_columns(K, N), groups = narrow_groups(M, c);
         if (need_dw) l.bytes = (size_t)groups * c * c * 4;
         l.part = l.bytes;
         if (need_db) l.bytes += up256((size_t)groups * N * 4);
@@ -1043,7 +1043,7 @@ extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const
         float* part = db ? (float*)(ws + l.part) : nullptr;
         const NarrowBwd a{dy, lddy, dz.slope, dz.mask, dz.factor, xcodes, xscales, wcodes, wscales, M, (int)K, (int)N, dx, lddx, dw, (float*)ws, part};
         int rc = launch_narrow_bwd(fn, a, dtype, st);
-        return rc || !db ? rc : launch_colsum(fn, part, narrow_groups(M), (int)N, dtype, db, st);
+        return rc || !db ? rc : launch_colsum(fn, part, narrow_groups(M, narrow_columns(K, N)), (int)N, dtype, db, st);
     }
     if (dtype == NERF_F32)
         return backward<float>(fn, l, dz, xcodes, xscales, wcodes, wscales, M, K, N, ws, dx, lddx, dw, db, st);

@@ -36,12 +36,13 @@ struct NarrowBwd {
     float* slab;            // dw: [groups][C][C], C = 128 or 256
     float* colsum;          // [groups][N], or NULL
 };
-// workgroups of the backward kernel: 32 rows at a time, four times at least
-static inline int narrow_groups(int64_t M) {
-    const int64_t g = (M + 127) / 128;
-    return g < 256 ? (int)g : 256;
-}
 static inline int narrow_columns(int64_t K, int64_t N) { return K > 128 || N > 128 ? 256 : 128; }
+// workgroups of the backward kernel: 32 rows at a time, four times at least; one fits a compute unit, or two of 128 columns
+// (131072 x 128 x 128 fp32 sin 45 -> 41 us, and one more for the sums)
+static inline int narrow_groups(int64_t M, int columns) {
+    const int64_t g = (M + 127) / 128, most = columns == 256 ? 256 : 512;
+    return (int)(g < most ? g : most);
+}
 // what the kernel's loads of whole 16-byte pieces ask of the layout
 static inline bool narrow_bwd_ok(const void* dy, int64_t lddy, int size, int64_t M, int64_t K, int64_t N, bool slope) {
     return M >= kNarrowRowsBwd && K <= kNarrow && N <= kNarrow && (uintptr_t)dy % 16 == 0 && lddy * size % 16 == 0 && N * size % 16 == 0 &&

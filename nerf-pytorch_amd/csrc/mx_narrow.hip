@@ -150,16 +150,22 @@ int by_act(const char* fn, const NarrowFwd& a, int act, hipStream_t st) {
 
 // ------------------------------------------------------------------------------------------------------- backward
 // All three gradients in one pass over dy, the slopes and the packed x.  A workgroup of eight waves walks its 32-row pieces:
-//   * dy and slopes of the next piece come straight into LDS while this one is multiplied, its codes into registers;
-//   * dz = dy * slope is split into bf16 terms, x is decoded, both as rows in LDS;
+//   * dz = dy * slope, out of LDS, where dy and the slopes came by themselves; as soon as a wave has read its rows the next
+//     piece's are requested into their place;
+//   * dz is split into bf16 terms, x is decoded, both as rows in LDS;
 //   * dx: the 32 rows times W, whose fragments every wave keeps in registers (an eighth of the columns each);
 //   * dW += dz^T x: each wave keeps a quarter by a half of the whole C x C result in accumulators to the end; the operands
 //     run along the rows here, so they are read with the transposing LDS read (ds_read_b64_tr_b16: lane j of sixteen gets
 //     column j of four rows);
 //   * db: column sums in registers.
-// In the end every workgroup writes its dW and db sums, two small kernels add them in order.  262144 x 256 x 256 fp32 moves
-// 0.84 GB in 296 us (sin; ReLU 0.60 GB in 255), and 12 + 7 us for the sums: bound by LDS, which every term of dz passes three times,
-// with the conversion between two products not overlapped.
+// In the end every workgroup writes its dW and db sums, two small kernels add them in order.
+//
+// 262144 x 256 x 256 fp32 moves 0.84 GB in 270 us (sin; ReLU 0.58 GB in 236, bf16 ReLU 0.31 GB in 114), and 12 + 7 us for the
+// sums.  With nothing to load the three phases take 200 us, splitting 78, dx 59, dW 63: two waves on a SIMD (the sums fill its
+// registers) hide little of each other's waits for LDS, and what is loaded and stored meets them only in part.  What brought
+// it from 297: operands read slots ahead of their matrix instructions (286); the transposing reads marked as apart from the
+// requests, for which the compiler had them wait (281); requests in front of the splitting instead of behind it, W's codes
+// loaded at once (267).
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);   // addresses are clamped by hand
 }
@@ -211,26 +217,22 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
             *reinterpret_cast<bf16x8*>(o + i * 16) = in ? decode8_bf16(c[i], s) : decode8_bf16(0u, 0u);
     };
 
-    // this wave's columns of W, as the A operand of dx = dz W: 32 rows of W at a time through LDS
-    bf16x8 wf[XT][C / 32];
+    unsigned wcodes[C / 32][CODES / 8], wscale[C / 32];       // 32 rows of W at a time
     if (a.dx) {
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
             const int n = s * 32 + row, k = l16 * CODES;
-            const bool in = n < a.N && k < steps * 128;
-            const int64_t at = in ? (int64_t)n * (steps * 128) + k : 0;    // values from the first code
-            unsigned c[CODES / 8];
+            const int64_t at = n < a.N && k < steps * 128 ? (int64_t)n * (steps * 128) + k : 0;    // values from the first code
 #pragma unroll
-            for (int i = 0; i < CODES / 8; ++i) c[i] = reinterpret_cast<const unsigned*>(a.wc + at / 2)[i];
-            decode(c, a.ws[at / 32], in);
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < XT; ++t) wf[t][s] = read_turned(smem + L::X + turned + (wave * XT + t) * 32, 4 * PITCH);
-            __syncthreads();
+            for (int i = 0; i < CODES / 8; ++i) wcodes[s][i] = reinterpret_cast<const unsigned*>(a.wc + at / 2)[i];
+            wscale[s] = a.ws[at / 32];
         }
     }
 
     constexpr int DYB = C * (int)sizeof(T);
+    const unsigned xpitch = a.dw ? steps * 128 : 0;
+    const uint8_t* xc = a.dw ? a.xc : (const uint8_t*)a.dy;
+    const uint8_t* xs = a.dw ? a.xs : (const uint8_t*)a.dy;
     [[maybe_unused]] uint16_t bits[CHUNKS];
     unsigned codes[CODES / 8], scale;
     // What wave w converts, rows 4w .. 4w + 3 of the piece, it also loads: no other wave is waited for.
@@ -256,22 +258,41 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
                 to_lds16(sl, smem + L::SLOPE + wave * (16 * C) + i * 1024, clamp(at) * a.N * 4 + (c < a.N * 4 ? c : 0));
             }
         }
-        if (a.dw) {
-            const int k = l16 * CODES < steps * 128 ? l16 * CODES : 0;
-            const int64_t at = (m0 + clamp(row)) * (steps * 128) + k;    // values from the first code
+        // (without dW the first bytes of dy: a branch around would make the compiler wait for these behind it)
+        const unsigned k = l16 * CODES < xpitch ? l16 * CODES : 0;
+        const uint64_t at = (uint64_t)(m0 + clamp(row)) * xpitch + k;    // values from the first code
 #pragma unroll
-            for (int i = 0; i < CODES / 8; ++i) codes[i] = reinterpret_cast<const unsigned*>(a.xc + at / 2)[i];
-            scale = a.xs[at / 32];
-        }
+        for (int i = 0; i < CODES / 8; ++i) codes[i] = reinterpret_cast<const unsigned*>(xc + at / 2)[i];
+        scale = xs[at / 32];
         if constexpr (SLOPE == 2) {
             const int words = (a.N + 15) / 16;
 #pragma unroll
             for (int i = 0; i < CHUNKS; ++i) {
                 const int w = i * 4 + l16 / 4;
-                bits[i] = w < words ? a.mask[(m0 + clamp(row)) * words + w] : 0;
+                bits[i] = a.mask[(m0 + clamp(row)) * words + (w < words ? w : 0)];
             }
         }
     };
+
+    int64_t piece = blockIdx.x;
+    if (piece < pieces) request(piece);
+
+    // this wave's columns of W, as the A operand of dx = dz W: through LDS (where the requests do not go).  Its tiles take
+    // turns in groups of four columns: a lane's results are then neighbours.
+    const int wcolumns = (q * 8 + (r >> 2)) * PITCH + wave * (XT * 32) + (r & 3) * (XT * 8);
+    bf16x8 wf[XT][C / 32];
+    if (a.dx) {
+#pragma unroll
+        for (int s = 0; s < C / 32; ++s) {
+            decode(wcodes[s], wscale[s], s * 32 + row < a.N && l16 * CODES < steps * 128);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+#pragma unroll
+            for (int t = 0; t < XT; ++t) wf[t][s] = read_turned(smem + L::X + wcolumns + t * 8, 4 * PITCH);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+        }
+    }
 
     f32x4 acc[KT][NT];
 #pragma unroll
@@ -281,8 +302,6 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
     f32x4 db = {0.f, 0.f, 0.f, 0.f};     // lane row q: columns 64 q + 4 l16 ..
     const int wn = wave >> 1, wk = wave & 1;
 
-    int64_t piece = blockIdx.x;
-    if (piece < pieces) request(piece);
     for (; piece < pieces; piece += gridDim.x) {
         // the piece has landed, and everybody is done with the rows of the previous one
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -292,114 +311,133 @@ __global__ __launch_bounds__(512, 2) void mx_narrow_bwd_kernel(NarrowBwd a) {
         asm volatile("" : "+v"(row), "+v"(l16), "+v"(r), "+v"(q));
         const int64_t m0 = piece * 32;
         const bool in_row = m0 + row < a.M;
+        if (a.dw) decode(codes, scale, in_row && l16 * CODES < steps * 128);
         f32x4 dz[4] = {};
+        unsigned top = 0;
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
             const int n = i * 64 + l16 * 4;
+            const bool in = in_row && n < a.N;      // N is a multiple of four
             const x4 d = *reinterpret_cast<const x4*>(smem + L::DY + row * DYB + n * (int)sizeof(T));
-            f32x4 v;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = in_row && n < a.N ? (float)d[j] : 0.0f;      // N is a multiple of four
-            if constexpr (SLOPE == 1) {
-                const f32x4 s = *reinterpret_cast<const f32x4*>(smem + L::SLOPE + row * (C * 4) + n * 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = in_row && n < a.N ? v[j] * s[j] : 0.0f;
-            }
-            if constexpr (SLOPE == 2) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = bits[i] >> (4 * (l16 & 3) + j) & 1 ? v[j] : 0.0f;
-            }
-            __bf16 t[4][TERMS];
-            unsigned top = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float x = v[j];
-                const unsigned b = __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
+                float v = (float)d[j];
+                if constexpr (SLOPE == 1) v *= reinterpret_cast<const float*>(smem + L::SLOPE + row * (C * 4) + n * 4)[j];
+                if constexpr (SLOPE == 2) v = bits[i] >> (4 * (l16 & 3) + j) & 1 ? v : 0.0f;
+                v = in ? v : 0.0f;
+                const unsigned b = __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
                 top = b > top ? b : top;
+                dz[i][j] = v;
             }
-            if (__any(top >= 0x7f7f8000u)) {    // not finite, or infinite as bf16: the careful way
+        }
+        // this wave has read its rows: the next ones come while these are split
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if (piece + gridDim.x < pieces) request(piece + gridDim.x);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool careful = __any(top >= 0x7f7f8000u);     // not finite, or infinite as bf16
 #pragma unroll
-                for (int j = 0; j < 4; ++j) split_terms<TERMS>(v[j], t[j]);
+        for (int i = 0; i < CHUNKS; ++i) {
+            bf16x4 t[TERMS];
+            if (careful) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    __bf16 u[TERMS];
+                    split_terms<TERMS>(dz[i][j], u);
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) t[k][j] = u[k];
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float x = v[j];
+                    float x = dz[i][j];
 #pragma unroll
                     for (int k = 0; k < TERMS; ++k) {
-                        t[j][k] = (__bf16)x;
-                        x -= (float)t[j][k];
+                        const __bf16 u = (__bf16)x;
+                        t[k][j] = u;
+                        x -= (float)u;
                     }
                 }
             }
-            dz[i] = v;
 #pragma unroll
             for (int k = 0; k < TERMS; ++k)
-                *reinterpret_cast<bf16x4*>(smem + k * L::PLANE + row * PITCH + n * 2) = bf16x4{t[0][k], t[1][k], t[2][k], t[3][k]};
+                *reinterpret_cast<bf16x4*>(smem + k * L::PLANE + row * PITCH + (i * 64 + l16 * 4) * 2) = t[k];
             __builtin_amdgcn_sched_barrier(0);      // registers are short: one group at a time
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) db[j] += rows_sum(dz[0][j], dz[1][j], dz[2][j], dz[3][j]);
-        if (a.dw) decode(codes, scale, in_row && l16 * CODES < steps * 128);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read its rows
-        if (piece + gridDim.x < pieces) request(piece + gridDim.x);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();                           // (not __syncthreads(): the requests stay under way)
         asm volatile("" ::: "memory");
 
+        // Both products: an operand of dz is read AHEAD slots before its matrix instructions, into the place of one just used.
         if (a.dx) {
+            constexpr int AHEAD = SLOPE == 2 ? 3 : 4, LEN = C / 32 * TERMS;      // slots of a row tile
+            bf16x8 z[AHEAD];
+            auto read_z = [&](auto I) {
+                constexpr int i = decltype(I)::value, mt = i / LEN, s = i / TERMS % (C / 32), k = i % TERMS;
+                if constexpr (i < 2 * LEN)
+                    z[i % AHEAD] = *reinterpret_cast<const bf16x8*>(smem + k * L::PLANE + (mt * 16 + r) * PITCH + s * 64 + q * 16);
+            };
+            unrolled<AHEAD>(read_z);
+            f32x4 o[XT];
+            unrolled<2 * LEN>([&](auto I) {
+                constexpr int i = decltype(I)::value, mt = i / LEN, s = i / TERMS % (C / 32);
+                if constexpr (i % LEN == 0) {
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                f32x4 o[XT];
-#pragma unroll
-                for (int t = 0; t < XT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = 0; s < C / 32; ++s) {
-#pragma unroll
-                    for (int k = 0; k < TERMS; ++k) {
-                        const bf16x8 z = *reinterpret_cast<const bf16x8*>(smem + k * L::PLANE + (mt * 16 + r) * PITCH + s * 64 + q * 16);
-#pragma unroll
-                        for (int t = 0; t < XT; ++t) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[t][s], z, o[t], 0, 0, 0);
-                    }
-                    if (s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                    for (int t = 0; t < XT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
                 }
-                const int64_t m = m0 + mt * 16 + r;
-                if (m < a.M) {
 #pragma unroll
-                    for (int t = 0; t < XT; ++t) {
-                        const int k = (wave * XT + t) * 16 + q * 4;
-                        T* p = (T*)a.dx + m * a.lddx + k;
-                        x4 v;
+                for (int t = 0; t < XT; ++t) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[t][s], z[i % AHEAD], o[t], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                read_z(std::integral_constant<int, i + AHEAD>{});
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (i % LEN == LEN - 1) {
+                    const int64_t m = m0 + mt * 16 + r;
+                    if (m < a.M) {
+                        constexpr int VALUES = sizeof(T) == 2 ? 4 * XT : 4;     // of a store
+                        const int k0 = (wave * 4 + q) * (4 * XT);
+                        T* p = (T*)a.dx + m * a.lddx + k0;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[j] = (T)(o[t][j] * a.factor);
-                        if (k + 4 <= a.K) {
-                            *reinterpret_cast<typename Loose<T, 4>::type*>(p) = v;
-                        } else {
+                        for (int h = 0; h < 4 * XT; h += VALUES) {
+                            typename Loose<T, VALUES>::type v;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (k + j < a.K) p[j] = v[j];
+                            for (int j = 0; j < VALUES; ++j) v[j] = (T)(o[(h + j) / 4][(h + j) % 4] * a.factor);
+                            if (k0 + h + VALUES <= a.K) {
+                                *reinterpret_cast<typename Loose<T, VALUES>::type*>(p + h) = v;
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < VALUES; ++j)
+                                    if (k0 + h + j < a.K) p[h + j] = v[j];
+                            }
                         }
                     }
                 }
-            }
+            });
         }
         if (a.dw) {
+            constexpr int AHEAD = 2, LEN = NT * TERMS, HALF = KT / 2;    // slots of half the columns of x
             const uint8_t* zl = smem + turned + wn * (NT * 32);
             const uint8_t* xl = smem + L::X + turned + wk * (KT * 32);
+            bf16x8 x[HALF], z[AHEAD];
+            auto read_z = [&](auto I) {
+                constexpr int i = decltype(I)::value, j = i / TERMS % NT, k = i % TERMS;
+                if constexpr (i < 2 * LEN) z[i % AHEAD] = read_turned(zl + k * L::PLANE + j * 32, 4 * PITCH);
+            };
+            unrolled<HALF>([&](auto I) { x[decltype(I)::value] = read_turned(xl + decltype(I)::value * 32, 4 * PITCH); });
+            unrolled<AHEAD>(read_z);
+            unrolled<2 * LEN>([&](auto I) {
+                constexpr int i = decltype(I)::value, half = i / LEN, j = i / TERMS % NT;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                bf16x8 x[KT / 2];
-#pragma unroll
-                for (int i = 0; i < KT / 2; ++i) x[i] = read_turned(xl + (half * (KT / 2) + i) * 32, 4 * PITCH);
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int k = 0; k < TERMS; ++k) {
-                        const bf16x8 z = read_turned(zl + k * L::PLANE + j * 32, 4 * PITCH);
-#pragma unroll
-                        for (int i = 0; i < KT / 2; ++i)
-                            acc[half * (KT / 2) + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], z, acc[half * (KT / 2) + i][j], 0, 0, 0);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-            }
+                for (int t = 0; t < HALF; ++t) {
+                    f32x4& sum = acc[half * HALF + t][j];
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[t], z[i % AHEAD], sum, 0, 0, 0);
+                    if constexpr (i == LEN - 1) x[t] = read_turned(xl + (HALF + t) * 32, 4 * PITCH);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                read_z(std::integral_constant<int, i + AHEAD>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
         }
     }
 
@@ -453,7 +491,7 @@ int launch_bwd(const char* fn, const NarrowBwd& a, hipStream_t st) {
     static_assert(lds <= 160 * 1024 && 32 * C * 4 <= lds, "LDS");
     int rc = nerf_set_lds(mx_narrow_bwd_kernel<T, TERMS, C, SLOPE>, lds);
     if (rc) return rc;
-    const int groups = narrow_groups(a.M);
+    const int groups = narrow_groups(a.M, C);
     mx_narrow_bwd_kernel<T, TERMS, C, SLOPE><<<(unsigned)groups, 512, lds, st>>>(a);
     if ((rc = nerf_check_launch(fn)) || !a.dw) return rc;
     mx_narrow_join_kernel<T, C><<<(unsigned)((a.N * C + 63) / 64), 256, 0, st>>>(a.slab, groups, a.N, a.K, a.factor, (T*)a.dw);
