@@ -130,11 +130,11 @@ struct FewArgs {
 };
 constexpr int kFewRows = 64;
 // Rows up to which a workgroup per sixteen columns, which reads x from the L2 each time, beats the tiles, which share it:
-// by what the workgroups read of x together and what a workgroup of the split product has to join.  Against the tiles, us,
-// K -> N: 4096 -> 4096 with 64 rows 10.4 : 12.0; 8192 -> 4096 with 32 11.7 : 12.6, with 48 15.2 : 13.3; 8192 -> 8192 with 16
+// sixteen (one tile row), or by what the workgroups read of x together and what a workgroup of the split product has to
+// join.  Against the tiles, us, K -> N: 4096 -> 4096 with 64 rows 10.4 : 12.0; 8192 -> 4096 with 32 11.7 : 12.6, with 48 15.2 : 13.3; 8192 -> 8192 with 16
 // 15.9 : 17.3, with 24 18.2 : 17.6, with 64 29.7 : 19.0; 1024 -> 16384 with 8 6.2 : 6.8, with 64 11.4 : 7.9.
 static inline bool few_rows(int64_t M, int64_t K, int64_t N) {
-    return M <= kFewRows && M * (K > N ? K : N) <= 1 << 18 && M * K * N <= 1 << 30;
+    return M <= 16 || (M <= kFewRows && M * (K > N ? K : N) <= 1 << 18 && M * K * N <= 1 << 30);
 }
 // One launch for both where every workgroup's rounding of x is short; a row has a cost of its own.  Against two launches,
 // us: 4096 -> 4096 with 1 row 4.6 : 5.9, with 4 5.7 : 6.2; 256 -> 256 with 24 4.3 : 5.1, with 64 6.3 : 5.6; 1024 -> 4096

@@ -950,7 +950,7 @@ extern "C" int nerf_mx_linear_fwd(const void* x, int dtype, int64_t ldx, const u
                  (long long)K, (long long)N, (long long)ldx, (long long)ldy);
     NERF_REQUIRE(dtype >= NERF_F32 && dtype <= NERF_F16, "%s: unknown type %d", fn, dtype);
     NERF_REQUIRE(act >= NERF_ACT_NONE && act <= NERF_ACT_SIGMOID, "%s: unknown activation %d", fn, act);
-    NERF_REQUIRE(!xcodes || M <= kTrainRows, "%s: more than 65535*64 rows kept for a backward pass", fn);
+    NERF_REQUIRE(!xcodes || (M <= kTrainRows && N <= kTrainRows), "%s: more than 65535*64 rows of x or W kept for a backward pass", fn);
     if (M == 0) return NERF_OK;
     NERF_REQUIRE_PTR(x);
     NERF_REQUIRE_PTR(wcodes);
@@ -1011,7 +1011,7 @@ extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const
                  (long long)M, (long long)K, (long long)N);
     NERF_REQUIRE(dtype >= NERF_F32 && dtype <= NERF_F16, "%s: unknown type %d", fn, dtype);
     NERF_REQUIRE(act >= NERF_ACT_NONE && act <= NERF_ACT_SIGMOID, "%s: unknown activation %d", fn, act);
-    NERF_REQUIRE(M <= kTrainRows, "%s: more than 65535*64 rows per call", fn);
+    NERF_REQUIRE(M <= kTrainRows && N <= kTrainRows, "%s: more than 65535*64 rows of x or W per call", fn);
     if (!dx && !dw && !db) return NERF_OK;
     NERF_REQUIRE_PTR(dy);
     NERF_REQUIRE_PTR(workspace);
@@ -1024,7 +1024,7 @@ extern "C" int nerf_mx_linear_bwd(const void* dy, int dtype, int64_t lddy, const
     const bool smooth = act == NERF_ACT_SIN || act == NERF_ACT_SIGMOID;
     const int size = dtype == NERF_F32 ? 4 : 2;
     const BwdLayout l = bwd_layout(dtype, act, M, K, N, dx != nullptr, dw != nullptr, db != nullptr,
-                                   narrow_bwd_ok(dy, lddy, size, M, K, N, smooth && slope));
+                                   narrow_bwd_ok(dy, lddy, size, M, K, N, smooth ? slope : nullptr));
     DzArgs dz{};
     dz.dy = dy;
     dz.lddy = lddy;

@@ -44,9 +44,9 @@ static inline int narrow_groups(int64_t M, int columns) {
     return (int)(g < most ? g : most);
 }
 // what the kernel's loads of whole 16-byte pieces ask of the layout
-static inline bool narrow_bwd_ok(const void* dy, int64_t lddy, int size, int64_t M, int64_t K, int64_t N, bool slope) {
+static inline bool narrow_bwd_ok(const void* dy, int64_t lddy, int size, int64_t M, int64_t K, int64_t N, const float* slope) {
     return M >= kNarrowRowsBwd && K <= kNarrow && N <= kNarrow && (uintptr_t)dy % 16 == 0 && lddy * size % 16 == 0 && N * size % 16 == 0 &&
-           (!slope || N % 4 == 0) && lddy <= (1 << 20);
+           (!slope || (N % 4 == 0 && (uintptr_t)slope % 16 == 0)) && lddy <= (1 << 20);
 }
 int launch_narrow_bwd(const char* fn, const NarrowBwd& a, int dtype, hipStream_t st);
 

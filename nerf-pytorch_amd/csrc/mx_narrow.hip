@@ -109,7 +109,7 @@ __global__ __launch_bounds__(512, 4) void mx_narrow_fwd_kernel(NarrowFwd a) {
             else a.xs[m * 4 + q] = (uint8_t)xs;
         }
         request(tile + stride);
-        constexpr int U = ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID ? 2 : 4;
+        constexpr int U = ACT == NERF_ACT_SIN || ACT == NERF_ACT_SIGMOID ? 1 : 4;
 #pragma unroll U
         for (int t = 0; t < ntiles; ++t) {
             const int row = t * 16 + r, n = t * 16 + q * 4;

@@ -176,7 +176,7 @@ def test_linear_many_tiles(dtype, act, M, K, N):
     check_forward(mx.linear(x, w, b, mx.ACTIVATIONS[act]), x, w, b, act, 1.0, 1.0)
 
 
-FEW = [(16, 8192, 8192), (17, 8192, 8192), (26, 256, 300), (28, 256, 300), (64, 4096, 4096), (64, 4100, 4096), (65, 512, 512), (8, 40, 33000)]
+FEW = [(16, 8192, 8192), (17, 8192, 8192), (26, 256, 300), (28, 256, 300), (64, 4096, 4096), (64, 4100, 4096), (65, 512, 512), (8, 40, 33000), (16, 130, 17000), (17, 130, 17000), (1, 130, 300000)]
 
 
 @pytest.mark.parametrize("M, K, N", FEW)
@@ -495,6 +495,39 @@ def test_other_stream():
     assert torch.equal(q, mx.dequantize(mx.quantize(x)))
 
 
+def test_gradients_at_odd_addresses():
+    """dy, slopes and decisions anywhere their types allow: the same bits as at aligned addresses."""
+    from nerf import _hip, mx
+    lib, M, K, N = _hip.lib, 4100, 64, 64
+    st = torch.cuda.current_stream().cuda_stream
+    x, w, dy = randn(M, K, seed=1), randn(N, K, seed=2), randn(M, N, seed=3)
+    for act in (mx.ACT_SIN, mx.ACT_RELU):
+        _, kept = _hip.mx_linear_train(x, w, None, None, act, 1.0, 1.0)
+        base = kept.buffer.data_ptr()
+        size = 4 * M * N if act == mx.ACT_SIN else 2 * M * (N // 16)
+        extra = torch.zeros(size + 16, dtype=torch.uint8, device=DEV)
+        at = 4 if act == mx.ACT_SIN else 2
+        extra[at:at + size] = kept.buffer[kept.extra:kept.extra + size]
+        odd = torch.zeros(M * N + 1, device=DEV)
+        odd[1:] = dy.view(-1)
+        ws = torch.empty(lib.nerf_mx_linear_bwd_workspace_bytes(0, act, M, K, N, 1, 1, 1), dtype=torch.uint8, device=DEV)
+        want = _hip.mx_linear_bwd(dy, kept, kept.buffer, None, True, True, True)
+        x64 = (np64(dy), np64(mx.dequantize(mx.quantize(x))), np64(mx.dequantize(mx.quantize(w))))
+        for dptr, eptr in ((odd.data_ptr() + 4, base + kept.extra), (dy.data_ptr(), extra.data_ptr() + at)):
+            dx, dw, db = torch.empty(M, K, device=DEV), torch.empty(N, K, device=DEV), torch.empty(N, device=DEV)
+            rc = lib.nerf_mx_linear_bwd(dptr, 0, N, eptr, eptr, act, 1.0, 1.0, base + kept.xcodes, base + kept.xscales, base + kept.wcodes,
+                                        base + kept.wscales, M, K, N, ws.data_ptr(), dx.data_ptr(), K, dw.data_ptr(), db.data_ptr(), st)
+            assert rc == 0
+            slope = np64(kept.buffer[kept.extra:kept.extra + size].view(torch.float32).view(M, N)) if act == mx.ACT_SIN else \
+                (np.unpackbits(kept.buffer[kept.extra:kept.extra + size].cpu().numpy().view(np.uint8), bitorder="little").reshape(M, N))
+            dz = x64[0] * slope
+            for got, same, exact, S, n in ((dx, want[0], dz @ x64[2], np.abs(dz) @ np.abs(x64[2]), N),
+                                           (dw, want[1], dz.T @ x64[1], np.abs(dz).T @ np.abs(x64[1]), M),
+                                           (db, want[2], dz.sum(0), np.abs(dz).sum(0), M)):
+                tol = (n + 4) * U * S + 2.0 ** -24 * np.abs(exact) + 2.0 ** -25 * S
+                assert (np.abs(np64(got) - exact) <= tol).all() and (np.abs(np64(same) - exact) <= tol).all()
+
+
 def test_two_calls_at_once():
     """The same layers forward and backward on two streams that run side by side, several times over."""
     sets = [(randn(m, k, seed=1), randn(n, k, seed=2), randn(n, seed=3), randn(m, n, seed=4))
@@ -547,6 +580,37 @@ def test_captured_and_replayed(M, K, N):
             torch.cuda.synchronize()
             assert torch.equal(out1, serve())
             assert all(torch.equal(a, c) for a, c in zip(out2, train()))
+
+
+@pytest.mark.parametrize("M, K, N", [(30, 96, 64), (5000, 96, 64)])
+def test_captured_through_autograd(M, K, N):
+    """Forward and torch.autograd.grad inside one capture (warmed up on another stream), replayed with new inputs."""
+    from nerf import mx
+    x, w, b, dy = randn(M, K, seed=1), randn(N, K, seed=2), randn(N, seed=3), randn(M, N, seed=4)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+
+    def step():
+        y = mx.linear(*leaves, mx.ACT_SIN)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(randn(M, K, seed=20 + i))
+            leaves[1].copy_(randn(N, K, seed=30 + i))
+            dy.copy_(randn(M, N, seed=40 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        y, grads = run_training(*leaves, dy, "sin")
+        assert torch.equal(out[0], y) and all(torch.equal(a, c) for a, c in zip(out[1:], grads))
 
 
 def test_a_run_of_layers_as_a_model_uses_them():

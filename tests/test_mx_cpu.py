@@ -93,6 +93,7 @@ def _fwd(**kw):
     (dict(M=1 << 30, N=1 << 22, ldy=1 << 22), -1, b"bad shape"), (dict(M=1 << 28), -1, b"bad shape"),
     (dict(M=1 << 19, N=1 << 22, ldy=1 << 22), -1, b"bad shape"),       # 2^32 threads
     (dict(xc=P, xs=P, M=65535 * 64 + 1), -1, b"kept for a backward pass"),
+    (dict(xc=P, xs=P, N=65535 * 64 + 1, ldy=1 << 23), -1, b"kept for a backward pass"),
     (dict(xc=P), -1, b"go together"), (dict(wc=P + 4), -1, b"aligned"), (dict(work=P + 8), -1, b"aligned"),
     (dict(M=0, x=None, y=None, work=None), 0, b""),
 ])
@@ -114,7 +115,8 @@ def _bwd(**kw):
     (dict(act=2), -2, b"slope is NULL"), (dict(act=3), -2, b"slope is NULL"), (dict(wc=None), -2, b"wcodes is NULL"),
     (dict(xs=None), -2, b"xscales is NULL"), (dict(lddy=7), -1, b"bad shape"), (dict(lddx=31), -1, b"bad shape"),
     (dict(M=0), -1, b"bad shape"), (dict(dtype=3), -1, b"unknown type 3"), (dict(act=9), -1, b"unknown activation 9"),
-    (dict(M=65535 * 64 + 1), -1, b"65535*64"), (dict(xc=P + 8), -1, b"aligned"),
+    (dict(M=65535 * 64 + 1), -1, b"65535*64"),
+    (dict(N=65535 * 64 + 1, lddy=1 << 23), -1, b"65535*64"), (dict(xc=P + 8), -1, b"aligned"),
     (dict(dx=None, dw=None, db=None, dy=None), 0, b""),
 ])
 def test_linear_bwd_refusals(kw, code, text):
