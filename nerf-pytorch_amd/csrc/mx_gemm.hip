@@ -326,6 +326,7 @@ __global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // two stages; PACKED: and two windows of scales
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const auto swizzle = [](int row) { return KIND == PACKED ? (row >> 1 & 1) | (row & 4) : row; };
     const int r = lane & 15, q = lane >> 4;
     int64_t m0;
     int n0;
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
     const uint8_t* from = op.p + first * op.pitch;
     const int size = valid * (int)op.pitch, ssize = valid * (int)op.sc_pitch;
     const uint8_t* sfrom = KIND == PACKED ? op.sc + first * op.sc_pitch : nullptr;
-    const int col = (lane & 7) ^ (lane >> 3);
+    const int col = (lane & 7) ^ swizzle(lane >> 3);
     int voff[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
         int w[NI], x[MI];
     } scales, next_scales;   // both halves' of a stage
     const int piece0 = KIND == PACKED ? 2 * q : q, piece1 = KIND == PACKED ? 2 * q + 1 : 4 + q;
-    const int place[2] = {r * 128 + ((piece0 ^ (r & 7)) * 16), r * 128 + ((piece1 ^ (r & 7)) * 16)};
+    const int place[2] = {r * 128 + ((piece0 ^ swizzle(r & 7)) * 16), r * 128 + ((piece1 ^ swizzle(r & 7)) * 16)};
     const int splace = 2 * STAGE + r * 16 + 2 * q;
     auto read_w = [&](auto I, auto HALF, i32x4 (&w)[NI], const uint8_t* stage) {
         w[decltype(I)::value] = *reinterpret_cast<const i32x4*>(stage + wn * 8192 + place[decltype(HALF)::value] + decltype(I)::value * 2048);
