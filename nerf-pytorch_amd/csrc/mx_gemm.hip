@@ -683,21 +683,28 @@ __global__ __launch_bounds__(256) void mx_colsum_kernel(const float* __restrict_
     }
 }
 
-// packed rows [rows][K] -> turned bf16 values [K][rows_p], zeros behind the last row.  Tiles of 64 rows x 128 values.
-__global__ __launch_bounds__(256) void mx_turn_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
-                                                     int64_t K, int64_t rows_p, __bf16* __restrict__ out) {
+// Packed rows [rows][K] -> turned bf16 values [K][rows_p], zeros behind the last row.  Tiles of 64 rows x 128 values; W and x
+// in one launch, neighbouring workgroups write neighbours.
+struct Turn {
+    const uint8_t *codes, *scales;
+    int64_t rows, rows_p;       // rows_p: 0 where there is nothing to turn
+    __bf16* out;
+};
+__global__ __launch_bounds__(256) void mx_turn_kernel(Turn first, Turn second, int64_t K) {
     constexpr int PITCH = 288;                              // bytes: 128 bf16 and 32 of padding
     __shared__ __attribute__((aligned(16))) uint8_t tile[64 * PITCH];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, q = lane >> 4;
-    const int64_t m0 = (int64_t)blockIdx.y * 64, k0 = (int64_t)blockIdx.x * 128;
+    const bool is_first = blockIdx.x < first.rows_p / 64;
+    const Turn& t = is_first ? first : second;
+    const int64_t m0 = ((int64_t)blockIdx.x - (is_first ? 0 : first.rows_p / 64)) * 64, k0 = (int64_t)blockIdx.y * 128;
     const int64_t m = m0 + (tid >> 2);
     u32x4 c = {0u, 0u, 0u, 0u};
     unsigned s = 0;
-    if (m < rows) {
+    if (m < t.rows) {
         const int64_t block = m * scale_pitch(K) + k0 / 32 + (tid & 3);
-        c = *reinterpret_cast<const u32x4*>(codes + block * 16);
-        s = scales[block];
+        c = *reinterpret_cast<const u32x4*>(t.codes + block * 16);
+        s = t.scales[block];
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -710,7 +717,7 @@ __global__ __launch_bounds__(256) void mx_turn_kernel(const uint8_t* __restrict_
         for (int h = 0; h < 2; ++h) {
             const bf16x8 v = read_turned(turned + j * 32 + h * (32 * PITCH), 4 * PITCH);
             const int64_t k = k0 + wave * 32 + j * 16 + r;
-            if (k < K) *reinterpret_cast<bf16x8*>(out + k * rows_p + m0 + h * 32 + q * 8) = v;
+            if (k < K) *reinterpret_cast<bf16x8*>(t.out + k * t.rows_p + m0 + h * 32 + q * 8) = v;
         }
 }
 
@@ -895,10 +902,12 @@ int backward(const char* fn, const BwdLayout& l, DzArgs dz, const uint8_t* xcode
     if ((dz.rows || dz.turned || dz.colsum) && (rc = launch_dz<T>(fn, dz, l.terms, st))) return rc;
     constexpr int dtype = sizeof(T) == 4 ? NERF_F32 : __is_same(T, __bf16) ? NERF_BF16 : NERF_F16;
     if (db && (rc = launch_colsum(fn, dz.colsum, (int)l.parts, (int)N, dtype, db, st))) return rc;
-    if (dx) {   // dx[m][k] = sum over n of dz[m][n] W[n][k]
-        mx_turn_kernel<<<dim3((unsigned)ceil_div64(K, 128), (unsigned)(l.Np / 64)), 256, 0, st>>>(wcodes, wscales, N, K, l.Np,
-                                                                                                 (__bf16*)(ws + l.wt));
+    const Turn w{wcodes, wscales, N, dx ? l.Np : 0, (__bf16*)(ws + l.wt)}, x{xcodes, xscales, M, dw ? l.Mp : 0, (__bf16*)(ws + l.xt)};
+    if (w.rows_p + x.rows_p) {
+        mx_turn_kernel<<<dim3((unsigned)((w.rows_p + x.rows_p) / 64), (unsigned)ceil_div64(K, 128)), 256, 0, st>>>(w, x, K);
         if ((rc = nerf_check_launch(fn))) return rc;
+    }
+    if (dx) {   // dx[m][k] = sum over n of dz[m][n] W[n][k]
         GemmArgs a{};
         a.w = Operand{ws + l.wt, l.Np * 2, nullptr, 0, K, 0};
         a.x = direct ? Operand{(const uint8_t*)dz.dy, dz.lddy * 2, nullptr, 0, M, 0} : Operand{ws + l.rows, l.Np * 2, nullptr, 0, M, M * l.Np * 2};
@@ -910,9 +919,6 @@ int backward(const char* fn, const BwdLayout& l, DzArgs dz, const uint8_t* xcode
         if ((rc = launch_gemm<BF16, T, NERF_ACT_NONE>(fn, a, l.dx, st))) return rc;
     }
     if (dw) {   // dW[n][k] = sum over m of dz[m][n] X[m][k]
-        mx_turn_kernel<<<dim3((unsigned)ceil_div64(K, 128), (unsigned)(l.Mp / 64)), 256, 0, st>>>(xcodes, xscales, M, K, l.Mp,
-                                                                                                 (__bf16*)(ws + l.xt));
-        if ((rc = nerf_check_launch(fn))) return rc;
         GemmArgs a{};
         a.w = Operand{ws + l.xt, l.Mp * 2, nullptr, 0, K, 0};
         a.x = Operand{ws + l.turned, l.Mp * 2, nullptr, 0, N, N * l.Mp * 2};
