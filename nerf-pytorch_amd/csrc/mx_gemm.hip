@@ -304,7 +304,9 @@ __device__ __forceinline__ void settle_all(f32x4 (&acc)[NI][MI]) {
 
 // The large tile: 256 x 256, eight waves of 128 (m) x 64 (n), two on each SIMD: what one wave waits for to issue -- a request,
 // a fragment read -- the other's matrix instructions hide.  (Four waves of 128 x 128 read a third less LDS, but alone on their
-// SIMDs took 51 us where this takes 47, packed 4096 x 4096 x 4096, and 146 where it takes 141, 4096 x 8192 x 8192.)  Stages as above, 128 bytes of each of the 512 rows, in two buffers.
+// SIMDs took 51 us where these took 47, packed 4096 x 4096 x 4096, and 146 where they took 141, 4096 x 8192 x 8192.)  Stages as
+// above, 128 bytes of each of the 512 rows, in two buffers.  Now 44 and 135 us (4.1 PFLOP/s): 1.7 us a stage and 15 a tile, 10
+// of those its stores, which leave all compute units together; bf16 4096 x 4096 x 4096 98 us (1.4 PFLOP/s).
 //
 // A stage's two halves are eight slots of four matrix instructions: slot j multiplies row fragment x[j] with the half's four
 // column fragments.  As soon as slot j is done, x[j] of the next half is read into its place, eight slots ahead; the column
@@ -315,7 +317,9 @@ __device__ __forceinline__ void settle_all(f32x4 (&acc)[NI][MI]) {
 // PACKED: the order of the blocks inside a stage is free as long as both operands agree, and lane group q takes blocks
 // 2q and 2q + 1 of the eight in its two halves: their two scale bytes are neighbours, one 16-bit read per row and stage,
 // and the matrix instruction picks the byte.  Scales are requested for two stages at a time, 16 bytes a row (8-byte
-// requests of 512 rows cost the L2 as much as the codes did); the last window of a row is moved back to end with it.
+// requests of 512 rows cost the L2 as much as the codes did); the last window of a row is moved back to end with it.  LDS serves
+// sixteen lanes at a time, of two neighbouring groups: with q and q + 1 in places 2q and 2q + 2 the permutation of a row is
+// another than for bf16 (half of the LDS cycles were conflicts before, 138 -> 135 us).
 //
 // Rows of 64 bytes a stage in a ring of four were slower: requests of half a cache line halve what the L2 delivers.
 template <int KIND, typename T, int ACT>
