@@ -232,6 +232,33 @@ def test_linear_takes_a_pitch_and_an_odd_address():
     check_forward(mx.linear(x, w), x, w, None, "none", 1.0, 1.0)
 
 
+@pytest.mark.parametrize("M", [5, 40, 300, 16400])
+@pytest.mark.parametrize("far", [0.0, 0.01, 0.5])
+def test_sines_of_large_arguments(M, far):
+    """Sums that are exact (codes times powers of two, small integers), times a power of two up to 2^20: sine and cosine of the
+    exact argument, a few, half or none of them beyond the short reduction's range, some infinite."""
+    from nerf import mx
+    K, N, g = 32, 40, torch.Generator().manual_seed(M)
+    x = torch.randint(0, 3, (M, K), generator=g).float()
+    x[torch.rand(M, generator=g) < far] *= 2.0 ** 8
+    w = torch.randint(-2, 3, (N, K), generator=g).float()
+    x, w = x.to(DEV), w.to(DEV)
+    assert torch.equal(mx.dequantize(mx.quantize(x)), x) and torch.equal(mx.dequantize(mx.quantize(w)), w)
+    pre = 2.0 ** 10
+    t = np64(x) @ np64(w).T * pre
+    assert (np.abs(t) < 2 ** 30).all() and (np.abs(t[0]) > 0).any()
+    xl = x.clone().requires_grad_(True)
+    y = mx.linear(xl, w, None, mx.ACT_SIN, pre, 2.0)
+    assert (np.abs(np64(y) - 2 * np.sin(t)) <= 2 * 8 * U).all()
+    (dx,) = torch.autograd.grad(y, xl, torch.ones_like(y))
+    want = (2 * pre * np.cos(t)) @ np64(w)
+    assert (np.abs(np64(dx) - want) <= 2 * pre * (8 + N) * U * np.abs(np64(w)).sum(0)).all()
+    x[1] = 2.0 ** 120
+    b = mx.linear(x, w, None, mx.ACT_SIN, 2.0 ** 20, 1.0)
+    over = np.abs(np64(x) @ np64(w).T) * 2.0 ** 20 > torch.finfo(torch.float32).max
+    assert torch.isnan(b)[torch.from_numpy(over).to(DEV)].all() and not torch.isnan(b[0]).any()
+
+
 def test_far_scales():
     """Blocks of very different magnitude: 2^-60 to 2^60 in one row (the products of the small ones vanish beside the sum)."""
     from nerf import mx
