@@ -500,6 +500,7 @@ def resample(weights: torch.Tensor, t_coarse: torch.Tensor, u: torch.Tensor, wan
 
 # --------------------------------------------------------------------------- microscaled 4-bit rows (nerf/mx.py)
 MX_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_U8 = torch.uint8
 
 
 def _mx_rows(t: torch.Tensor, name: str):
@@ -533,17 +534,18 @@ def mx_packed_shape(rows: int, K: int):
 
 def _mx_packed(codes: torch.Tensor, scales: torch.Tensor, K: int, device, name: str):
     """Pointers of packed rows of K values on `device`."""
-    c, s = mx_packed_shape(codes.shape[0], K)
-    if codes.shape != c or scales.shape != s:
+    if (codes.shape, scales.shape) != mx_packed_shape(codes.shape[0], K):
         raise ValueError(f"{name}: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} are not packed rows of {K} values")
     if codes.device != device or scales.device != device:
         raise ValueError(f"{name}: codes and scales must be on {device}")
-    return _dev(codes, f"{name}.codes", torch.uint8), _dev(scales, f"{name}.scales", torch.uint8)
+    if codes.dtype is _U8 and scales.dtype is _U8 and codes.is_cuda and codes.is_contiguous() and scales.is_contiguous():
+        return codes.data_ptr(), scales.data_ptr()
+    return _dev(codes, f"{name}.codes", torch.uint8), _dev(scales, f"{name}.scales", torch.uint8)    # says what is wrong
 
 
 def _mx_alloc(rows: int, K: int, like: torch.Tensor):
     c, s = mx_packed_shape(rows, K)
-    return like.new_empty(c, dtype=torch.uint8), like.new_empty(s, dtype=torch.uint8)
+    return like.new_empty(c, dtype=_U8), like.new_empty(s, dtype=_U8)
 
 
 def mx_quantize(x: torch.Tensor):

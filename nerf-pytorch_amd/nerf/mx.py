@@ -43,6 +43,8 @@ class MXTensor(NamedTuple):
 
 def _matrix(x: Tensor, name: str) -> Tensor:
     """[.., K] as a matrix with contiguous rows; a view where the layout allows it."""
+    if x.dim() == 2 and x.is_contiguous() and x.shape[1]:
+        return x
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"{name}: expected rows of at least one value, got shape {tuple(x.shape)}")
     if x.dim() != 2:
@@ -55,7 +57,7 @@ def _matrix(x: Tensor, name: str) -> Tensor:
 def quantize(x: Tensor) -> MXTensor:
     """Packed rows of x [.., K] (float32, bfloat16, float16; leading dimensions are flattened).  Not differentiable: the
     gradient of a layer goes through `linear`."""
-    m = _matrix(x.detach(), "x")
+    m = _matrix(x, "x")
     return MXTensor(*_hip.mx_quantize(m), m.shape[1])
 
 
@@ -91,6 +93,6 @@ def linear(x: Tensor, weight: Union[MXTensor, Tensor], bias: Optional[Tensor] = 
         y = MXLinearFunction.apply(m, W, packed, bias, act, float(pre), float(post))
     else:
         if packed is None:
-            packed = _hip.mx_quantize(W.detach())
-        y = _hip.mx_linear_fwd(m.detach(), *packed, None if bias is None else bias.detach(), act, pre, post)
+            packed = _hip.mx_quantize(W)
+        y = _hip.mx_linear_fwd(m, *packed, bias, act, pre, post)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
