@@ -9,7 +9,7 @@
 // The gradients are those of the product at the rounded operands (straight through the rounding).  X and W as they were
 // rounded are exact in bf16 (a code times a power of two); dz goes in as `terms` bf16 terms (dz = t0 + t1 + t2, each the
 // rounding of what the previous ones left): one for bf16 dy without a smooth activation (exact), two for fp16 dy (11 bits:
-// exact) and for bf16 dy through sin / sigmoid (2^-17, far under the output's own rounding), three for fp32 (exact up to
+// exact) and for 16-bit dy through sin / sigmoid (2^-17, far under the output's own rounding), three for fp32 (exact up to
 // 2^-25).  Sums are fp32 throughout; a split reduction writes fp32 slabs that a second kernel adds in a fixed order.
 #include "mx_narrow.h"
 
