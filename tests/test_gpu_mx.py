@@ -555,6 +555,44 @@ def test_gradients_at_odd_addresses():
                 assert (np.abs(np64(got) - exact) <= tol).all() and (np.abs(np64(same) - exact) <= tol).all()
 
 
+def test_products_beyond_32_bits():
+    """Outputs and operands of more than 2^32 bytes and 2^31 values: the last rows are those of a small call."""
+    from nerf import _hip, mx
+    # tiles: 2.3e9 outputs with their slopes (one step along the rows, so the order of the sums is the same everywhere)
+    M, K, N = 70000, 40, 32800
+    x, w = randn(M, K, seed=1, dtype=torch.bfloat16), randn(N, K, seed=2, dtype=torch.bfloat16)
+    y, kept = _hip.mx_linear_train(x, w, None, None, mx.ACT_SIN, 1.0, 1.0)
+    small, few = _hip.mx_linear_train(x[-300:], w, None, None, mx.ACT_SIN, 1.0, 1.0)
+    assert torch.equal(y[-300:], small)
+    assert torch.equal(kept.buffer[kept.extra + 4 * (M - 300) * N:kept.extra + 4 * M * N], few.buffer[few.extra:few.extra + 4 * 300 * N])
+    del y, kept, small, few, x, w
+    # narrow and general gradients at the most rows a call trains; only the last rows have an upstream gradient
+    M, tail = 65535 * 64, 16384
+    for K, N, dtype in ((256, 256, torch.float32), (40, 300, torch.float32), (40, 300, torch.bfloat16)):
+        x = torch.zeros(M, K, dtype=dtype, device=DEV)
+        x[-tail:] = randn(tail, K, seed=3, dtype=dtype)
+        dy = torch.zeros(M, N, dtype=dtype, device=DEV)
+        dy[-tail:] = randn(tail, N, seed=4, dtype=dtype)
+        w = randn(N, K, seed=5, dtype=dtype)
+        y, kept = _hip.mx_linear_train(x, w, None, None, mx.ACT_SIN, 1.0, 1.0)
+        dx, dw, db = _hip.mx_linear_bwd(dy, kept, kept.buffer, None, True, True, True)
+        assert not dx[:-tail].any()
+        xt, dyt = x[-tail:].clone(), dy[-tail:].clone()
+        del x, dy, kept
+        ys, kept = _hip.mx_linear_train(xt, w, None, None, mx.ACT_SIN, 1.0, 1.0)
+        dxs, dws, dbs = _hip.mx_linear_bwd(dyt, kept, kept.buffer, None, True, True, True)
+        eps = torch.finfo(dtype).eps
+        X64, W64 = mx.dequantize(mx.quantize(xt)).double().abs(), mx.dequantize(mx.quantize(w)).double().abs()
+        z = X64 @ W64.t()
+        # |dz| <= |dy|; the two calls sum in other orders, in y's case inside the argument of the sine as well
+        assert ((y[-tail:] - ys).double().abs() <= 2 * (K + 2) * U * z + 8 * U + eps * ys.double().abs()).all()
+        dz, ez = dyt.double().abs(), dyt.double().abs() * (2 * (K + 2) * U * z + 8 * U)
+        for got, want, S, E, n in ((dx[-tail:], dxs, dz @ W64, ez @ W64, N), (dw, dws, dz.t() @ X64, ez.t() @ X64, tail),
+                                   (db, dbs, dz.sum(0), ez.sum(0), tail)):
+            assert ((got - want).double().abs() <= E + (2 * (3 * n + 8) * U + 2.0 ** -16) * S + eps * want.double().abs()).all()
+        del y, dx, ys, kept
+
+
 def test_two_calls_at_once():
     """The same layers forward and backward on two streams that run side by side, several times over."""
     sets = [(randn(m, k, seed=1), randn(n, k, seed=2), randn(n, seed=3), randn(m, n, seed=4))
