@@ -6,9 +6,10 @@ namespace mxk {
 
 constexpr int kNarrow = 256;            // inputs and outputs
 // Rows from which the fixed cost (weights read back, partial sums) is less than the bytes and launches that are saved.
-// Against the general way, us: forward 256 -> 256 relu fp32 with 8192 rows 11.3 : 8.2, 16384 13.6 : 14.4; sin fp32 with 12288
-// 17.7 : 11.6, 16384 18.5 : 18.7, 32768 23.1 : 23.6; 64 -> 64 with 32768 9.0 : 17.8.  Backward 256 -> 256 sin fp32 with 1024
-// 38.7 : 32.0, 4096 43.0 : 42.1, 8192 47.5 : 50.2, 65536 87 : 287; 64 -> 64 with 4096 19.9 : 24.9.
+// Against the general way, us: forward 256 -> 256 relu fp32 with 8192 rows 11.3 : 8.1, 16384 13.3 : 14.1; sin fp32 with 12288
+// 16.2 : 10.7, 16384 16.7 : 17.2, 32768 21.4 : 22.5; 64 -> 64 sin fp32 with 32768 8.6 : 15.5.  Backward 256 -> 256 sin fp32 with
+// 4096 39.9 : 40.1, 8192 44.4 : 48.6, 32768 57 : 117, relu bf16 with 4096 31.0 : 28.3, 8192 36.0 : 35.3, 32768 47 : 63; 64 -> 64
+// sin fp32 with 4096 18.0 : 23.2.
 constexpr int64_t kNarrowRowsFwd = 16384, kNarrowRowsBwd = 4096;
 
 struct NarrowFwd {
