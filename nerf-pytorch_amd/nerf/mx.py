@@ -21,6 +21,7 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _hip
 from ._hip import ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SIN
@@ -72,7 +73,8 @@ def linear(x: Tensor, weight: Union[MXTensor, Tensor], bias: Optional[Tensor] = 
 
     weight: packed rows (MXTensor), or a float tensor [N,K] of x's type that the call quantises.  act: ACT_NONE, ACT_RELU,
     ACT_SIN or ACT_SIGMOID.  Differentiable in x, a float weight and the bias: the gradients of the product at the rounded
-    operands, straight through the rounding (first order only)."""
+    operands, straight through the rounding (first order, reverse mode only: a tangent of forward-mode differentiation is
+    refused)."""
     if isinstance(weight, MXTensor):
         K, N, packed, W = weight.K, weight.rows, (weight.codes, weight.scales), None
     else:
@@ -86,6 +88,10 @@ def linear(x: Tensor, weight: Union[MXTensor, Tensor], bias: Optional[Tensor] = 
         raise ValueError(f"x {tuple(x.shape)} does not end with the weight's {K} values per row")
     if act not in (ACT_NONE, ACT_RELU, ACT_SIN, ACT_SIGMOID):
         raise ValueError(f"unknown activation {act}")
+    if forward_ad._current_level >= 0:      # inside a dual_level; tangents do not show in requires_grad
+        for t in (x, W, bias):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("mx.linear has no forward-mode derivative")
     m = _matrix(x, "x")
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()

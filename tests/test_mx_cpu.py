@@ -176,3 +176,30 @@ def test_models_and_commands_know_the_mode():
     assert _fused_model(m)
     m.set_training_precision("mxfp4")
     assert not _fused_model(m)
+
+
+@pytest.mark.parametrize("packed, dual", [(False, "x"), (False, "weight"), (False, "bias"), (True, "x"), (True, "bias")])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(monkeypatch, packed, dual, grad):
+    """A tangent on any operand is refused, whether or not gradients are recorded: it would be lost without a word.  (The
+    kernels are replaced: this runs without a GPU, and nothing may reach them.)"""
+    import torch.autograd.forward_ad as fwd
+    from nerf import _hip, mx
+    calls = []
+    monkeypatch.setattr(_hip, "mx_linear_fwd", lambda x, wc, *a: calls.append("fwd") or x.new_zeros(x.shape[0], wc.shape[0]))
+    monkeypatch.setattr(_hip, "mx_quantize", lambda w: (torch.zeros(w.shape[0], 64, dtype=torch.uint8), None))
+    monkeypatch.setattr(mx.MXLinearFunction, "apply", lambda x, w, *a: calls.append("train") or x.new_zeros(x.shape[0], 8))
+    t = {"x": torch.ones(4, 32, requires_grad=grad), "weight": torch.ones(8, 32), "bias": torch.ones(8)}
+    q = mx.MXTensor(torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.uint8), 32)
+    with fwd.dual_level():
+        plain = dict(t)
+        t[dual] = fwd.make_dual(t[dual], torch.ones_like(t[dual]))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    mx.linear(t["x"], q if packed else t["weight"], t["bias"])
+        assert not calls
+        mx.linear(plain["x"], q if packed else plain["weight"], plain["bias"])      # no tangent: the level alone changes nothing
+        assert calls == ["train" if grad else "fwd"]
+    mx.linear(plain["x"], q if packed else plain["weight"], None)
+    assert calls[1:] == ["train" if grad else "fwd"]
