@@ -11,6 +11,7 @@
 // rounding of what the previous ones left): one for bf16 dy without a smooth activation (exact), two for fp16 dy (11 bits:
 // exact) and for 16-bit dy through sin / sigmoid (2^-17, far under the output's own rounding), three for fp32 (exact up to
 // 2^-25).  Sums are fp32 throughout; a split reduction writes fp32 slabs that a second kernel adds in a fixed order.
+#include "mx_large.h"
 #include "mx_narrow.h"
 
 namespace mxk {
@@ -324,9 +325,9 @@ __device__ __forceinline__ void settle_all(f32x4 (&acc)[NI][MI]) {
 // Rows of 64 bytes a stage in a ring of four were slower: requests of half a cache line halve what the L2 delivers.
 template <int KIND, typename T, int ACT>
 __global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
-    constexpr int TILE = 256, R = 512, NI = 4, MI = 8;
+    constexpr int TILE = 256, NI = 4, MI = 8;
     constexpr int PIECES = 8;               // requests of a wave per stage
-    constexpr int STAGE = R * 128, SCALES = R * 16;
+    constexpr int STAGE = LargeLds::STAGE, SCALES = LargeLds::SCALES;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // two stages; PACKED: and two windows of scales
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
     } scales, next_scales;   // both halves' of a stage
     const int piece0 = KIND == PACKED ? 2 * q : q, piece1 = KIND == PACKED ? 2 * q + 1 : 4 + q;
     const int place[2] = {r * 128 + ((piece0 ^ swizzle(r & 7)) * 16), r * 128 + ((piece1 ^ swizzle(r & 7)) * 16)};
-    const int splace = 2 * STAGE + r * 16 + 2 * q;
+    const int splace = LargeLds::scale_place(r, q);
     auto read_w = [&](auto I, auto HALF, i32x4 (&w)[NI], const uint8_t* stage) {
         w[decltype(I)::value] = *reinterpret_cast<const i32x4*>(stage + wn * 8192 + place[decltype(HALF)::value] + decltype(I)::value * 2048);
     };
@@ -410,11 +411,6 @@ __global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
             if constexpr (i < NI) sc.w[i] = *reinterpret_cast<const uint16_t*>(smem + splace + scale_at + wn * 1024 + i * 256);
             else sc.x[i - NI] = *reinterpret_cast<const uint16_t*>(smem + splace + scale_at + 4096 + wm * 2048 + (i - NI) * 256);
         }
-    };
-    // where the scales of stage d are: their window, and inside it (moved back by what the last window was)
-    auto scales_of = [&](int d) {
-        const int window = (d >> 1) * 16, end = a.steps * 4 - 16;
-        return (d >> 1 & 1) * SCALES + (d & 1) * 8 + (window > end ? window - end : 0);
     };
     auto slot = [&](auto J, auto HALF, const i32x4 (&w)[NI]) {
         constexpr int j = decltype(J)::value, half = decltype(HALF)::value;
@@ -462,7 +458,7 @@ __global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
             if (KIND == PACKED && odd && d == D - 1) blank(w1);
         Request rq;
         if constexpr (REQUEST) rq = request(d + 2);
-        const int scale_at = scales_of(d + 1);
+        const int scale_at = LargeLds::scales_of(a.steps, d + 1);
         __builtin_amdgcn_sched_barrier(0);
         unrolled<MI>([&](auto J) {
             constexpr int j = decltype(J)::value;
@@ -493,7 +489,7 @@ __global__ __launch_bounds__(512, 2) void mx_gemm_large_kernel(GemmArgs a) {
     }
     unrolled<NI>([&](auto I) { read_w(I, H0, w0, smem); });
     unrolled<MI>([&](auto J) { read_x(J, H0, smem); });
-    unrolled<NI + MI>([&](auto I) { read_scale(I, scales, scales_of(0)); });
+    unrolled<NI + MI>([&](auto I) { read_scale(I, scales, LargeLds::scales_of(a.steps, 0)); });
     int d = 0;   // (behind the last stage old contents are read, and not used)
     for (; d + 2 < D; ++d) stage_body(std::true_type{}, d);
     for (; d < D; ++d) stage_body(std::false_type{}, d);
@@ -774,7 +770,7 @@ int launch_gemm_tile(const char* fn, const GemmArgs& a, int splits, hipStream_t 
 
 template <int KIND, typename T, int ACT>
 int launch_gemm_large(const char* fn, const GemmArgs& a, int splits, hipStream_t st) {
-    constexpr int lds = 2 * (512 * 128 + (KIND == PACKED ? 512 * 16 : 0));
+    constexpr int lds = LargeLds::bytes(KIND == PACKED);
     int rc = nerf_set_lds(mx_gemm_large_kernel<KIND, T, ACT>, lds);
     if (rc) return rc;
     mx_gemm_large_kernel<KIND, T, ACT><<<dim3((unsigned)(a.tiles_m * a.tiles_n), 1, (unsigned)splits), 512, lds, st>>>(a);

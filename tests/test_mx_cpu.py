@@ -203,3 +203,14 @@ def test_forward_mode_is_refused(monkeypatch, packed, dual, grad):
         assert calls == ["train" if grad else "fwd"]
     mx.linear(plain["x"], q if packed else plain["weight"], None)
     assert calls[1:] == ["train" if grad else "fwd"]
+
+
+def test_large_tile_reads_its_scales_inside_lds(tmp_path):
+    """The addresses of the large packed tile's scales (csrc/mx_large.h), followed on the host for all lengths of a row."""
+    import os
+    import subprocess
+    exe = tmp_path / "lds"
+    source = os.path.join(os.path.dirname(os.path.abspath(__file__)), "host", "mx_large_lds.cpp")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", "-o", str(exe), source], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
