@@ -89,3 +89,79 @@ def test_bf16_rows_of_dy_are_read_in_place():
             rows[:, :N] = dy
             got, _ = backward_entry(kept, rows, pitch, (1, 1, 1))
             assert all(torch.equal(a, c) for a, c in zip(got, want)), (M, pitch, shift)
+
+
+# ------------------------------------------------------------------------------------ the ends of the range, NaN, infinities
+@pytest.mark.parametrize("act", ["none", "relu", "sin"])
+@pytest.mark.parametrize("M, K, N", [(70, 64, 32), (4200, 64, 32), (4200, 200, 256), (700, 300, 320)])
+def test_upstream_gradients_at_the_end_of_the_range(act, M, K, N):
+    """Values above the largest bf16, whose first term would round to infinity: dx and dW, which are made of the terms, against
+    float64.  x and w are small enough for the true results to stay finite."""
+    from nerf import _hip, mx
+    top = torch.finfo(torch.float32).max
+    x, w = randn(M, K, seed=51, scale=2.0 ** -10), randn(N, K, seed=52, scale=2.0 ** -12)
+    b = torch.sign(randn(N, seed=53)).clamp(min=0 if act == "relu" else -1) * (30.0 if act == "relu" else 0.0)
+    if act == "relu":
+        b[b == 0] = -30.0
+        b[[3, 5, N - 1]] = 30.0
+    dy = randn(M, N, seed=54)
+    for m, n, v in ((2, 3, top), (M - 1, N - 1, -top), (M // 2, 5, 0.9985 * top), (33, 0, -0.9999 * top)):
+        dy[m, n] = v
+    assert (dy.abs() > 3.3895e38).sum() == 4 and torch.isinf(dy.to(torch.bfloat16)).sum() == 4
+    y, grads = run_training(x, w, b, dy, act)
+    assert all(torch.isfinite(g).all() for g in grads)
+    assert float(grads[0][2].abs().max()) > 1e33 and float(grads[1][3].abs().max()) > 1e33
+    check_backward(grads, dy, x, w, b, act, 1.0, 1.0, torch.float32)
+    _, kept = _hip.mx_linear_train(x, w, None, b, mx.ACTIVATIONS[act], 1.0, 1.0)
+    assert is_narrow(kept, dy, N) == (M >= 4096)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, K, N", [(70, 200, 64), (4200, 200, 64), (4101, 255, 248)])
+def test_unfinite_upstream_gradients_stay_in_their_row_and_column(dtype, M, K, N):
+    for act in ("none", "sin"):
+        x, w, b, dy = training_case(M, K, N, act, dtype)
+        clean = run_training(x, w, b, dy, act)[1]
+        bad = dy.clone()
+        bad[2, 3], bad[M - 1, N - 1], bad[40, 6] = float("inf"), float("nan"), float("-inf")
+        dx, dw, db = run_training(x, w, b, bad, act)[1]
+        rows, cols = torch.ones(M, dtype=torch.bool), torch.ones(N, dtype=torch.bool)
+        rows[[2, M - 1, 40]], cols[[3, N - 1, 6]] = False, False
+        assert torch.equal(dx[rows], clean[0][rows]) and torch.equal(dw[cols], clean[1][cols]) and torch.equal(db[cols], clean[2][cols])
+        assert not torch.isfinite(dx[~rows]).any() and not torch.isfinite(dw[~cols]).any() and not torch.isfinite(db[~cols]).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, K, N", [(70, 200, 64), (4200, 200, 64), (3400, 900, 200)])
+def test_nan_blocks_reach_the_gradients_they_feed(dtype, M, K, N):
+    """A block of x that is NaN: its 32 columns of dW, nothing else.  A block of W: its 32 columns of dx."""
+    x, w, b, dy = training_case(M, K, N, "none", dtype)
+    dx, dw, db = run_training(x, w, b, dy, "none")[1]
+    k0 = K // 32 * 32          # the last, incomplete block
+    assert k0 < K
+    xn, wn = x.clone(), w.clone()
+    xn[M - 1, K - 1], wn[5, 40] = float("inf"), float("nan")
+    ex, ew, eb = run_training(xn, w, b, dy, "none")[1]
+    assert torch.equal(ex, dx) and torch.equal(eb, db) and torch.equal(ew[:, :k0], dw[:, :k0]) and torch.isnan(ew[:, k0:]).all()
+    ex, ew, eb = run_training(x, wn, b, dy, "none")[1]
+    assert torch.equal(ew, dw) and torch.equal(eb, db) and torch.isnan(ex[:, 32:64]).all()
+    keep = [k for k in range(K) if not 32 <= k < 64]
+    assert torch.equal(ex[:, keep], dx[:, keep])
+
+
+@pytest.mark.parametrize("M, K, N", [(16400, 200, 40), (16390, 100, 130), (3400, 1100, 3601), (3400, 520, 3601), (4000, 900, 2200)])
+@pytest.mark.parametrize("act", ACTS)
+def test_nan_stays_in_its_row_or_column_of_many_rows(act, M, K, N):
+    """The pass for narrow layers, and tiles: the large one with nine and five steps has the poisoned blocks in the last stage,
+    half of which does not exist."""
+    from nerf import mx
+    x, w = randn(M, K, seed=12), randn(N, K, seed=13, scale=K ** -0.5)
+    clean = mx.linear(x, w, None, mx.ACTIVATIONS[act])
+    xn, wn = x.clone(), w.clone()
+    xn[M - 1, K - 1] = float("inf")
+    y = mx.linear(xn, w, None, mx.ACTIVATIONS[act])
+    assert torch.isnan(y[M - 1]).all() and torch.equal(y[:M - 1], clean[:M - 1])
+    wn[3, K - 1], wn[N - 1, 0] = float("nan"), float("-inf")
+    y = mx.linear(x, wn, None, mx.ACTIVATIONS[act])
+    keep = [n for n in range(N) if n not in (3, N - 1)]
+    assert torch.isnan(y[:, [3, N - 1]]).all() and torch.equal(y[:, keep], clean[:, keep])
