@@ -165,3 +165,56 @@ def test_nan_stays_in_its_row_or_column_of_many_rows(act, M, K, N):
     y = mx.linear(x, wn, None, mx.ACTIVATIONS[act])
     keep = [n for n in range(N) if n not in (3, N - 1)]
     assert torch.isnan(y[:, [3, N - 1]]).all() and torch.equal(y[:, keep], clean[:, keep])
+
+
+# ------------------------------------------------------------------------------------------------------------ the large tile
+@pytest.mark.parametrize("dtype, act, K", [
+    (torch.float32, "relu", 512), (torch.bfloat16, "none", 512), (torch.float32, "sin", 385), (torch.float16, "sigmoid", 400),
+    (torch.float32, "relu", 800), (torch.bfloat16, "relu", 897), (torch.float16, "none", 897), (torch.float32, "none", 1024),
+    (torch.bfloat16, "sin", 1024), (torch.float32, "relu", 1153)])
+def test_large_tile_from_four_steps(dtype, act, K):
+    """14 x 15 tiles of 256 x 256, ragged at both edges, four to ten steps of 128 values along the rows: two stages with one window
+    of scales, windows moved back to the row's end, last stages that exist by half."""
+    from nerf import mx
+    M, N = 3400, 3601
+    x, w, b, _ = training_case(M, K, N, "none", dtype)
+    y = mx.linear(x, w, b, mx.ACTIVATIONS[act])
+    check_forward(y, x, w, b, act, 1.0, 1.0)
+
+
+@pytest.mark.parametrize("M, K, N", [(3400, 512, 3601), (3400, 650, 3601), (16400, 200, 250), (16387, 70, 33), (300, 200, 75), (4000, 900, 2200)])
+def test_relu_masks_of_every_tile(M, K, N):
+    """Mixed decisions: the gradient is open exactly where y > 0 (column sums of ones: whole numbers, exact)."""
+    from nerf import mx
+    x, w = randn(M, K, seed=35), randn(N, K, seed=36)
+    b = torch.zeros(N, device=DEV, requires_grad=True)
+    y = mx.linear(x, w, b, mx.ACT_RELU)
+    (db,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    assert torch.equal(db, (y > 0).float().sum(0)) and 0 < float(db.min()) and float(db.max()) < M
+
+
+def test_training_relu_through_the_large_tile():
+    x, w, b, dy = training_case(3400, 512, 3601, "relu", torch.float32)
+    y, grads = run_training(x, w, b, dy, "relu", 0.5, 3.0)
+    check_forward(y, x, w, b, "relu", 0.5, 3.0)
+    check_backward(grads, dy, x, w, b, "relu", 0.5, 3.0, torch.float32)
+
+
+# ---------------------------------------------------------------------------------------------------------------- layouts
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, K, N", [(1, 1000, 40), (13, 500, 40), (40, 4100, 300), (300, 319, 257), (16400, 200, 40), (3400, 650, 3601)])
+def test_what_lies_between_rows_is_not_read(dtype, M, K, N):
+    """x with NaN between its rows, at an odd address, in every way to multiply and in the rounding."""
+    from nerf import mx
+    x, w = randn(M, K, seed=1, dtype=dtype), randn(N, K, seed=2, dtype=dtype)
+    buf = torch.full((M * (K + 7) + 3,), float("nan"), dtype=dtype, device=DEV)
+    rows = buf[3:].view(M, K + 7)
+    rows[:, :K] = x
+    q = mx.quantize(w)
+    assert torch.equal(mx.linear(rows[:, :K], q), mx.linear(x, q))
+    a, c = mx.quantize(rows[:, :K]), mx.quantize(x)
+    assert torch.equal(a.codes, c.codes) and torch.equal(a.scales, c.scales)
+    part = slice(N // 3, N)     # some of the rows of a packed weight are packed rows
+    some = mx.MXTensor(q.codes[part], q.scales[part], K)
+    want = mx.linear(x, mx.quantize(w[part]))
+    assert torch.equal(mx.linear(x, some), want) and torch.equal(mx.dequantize(some), mx.dequantize(q)[part])
