@@ -218,3 +218,45 @@ def test_what_lies_between_rows_is_not_read(dtype, M, K, N):
     some = mx.MXTensor(q.codes[part], q.scales[part], K)
     want = mx.linear(x, mx.quantize(w[part]))
     assert torch.equal(mx.linear(x, some), want) and torch.equal(mx.dequantize(some), mx.dequantize(q)[part])
+
+
+# ------------------------------------------------------------------------------------------------------------ data parallel
+@pytest.mark.parametrize("tag", ["nerf", "siren"])
+def test_flat_bucket_holds_the_mean_over_ranks(tag, monkeypatch):
+    """Data-parallel training in the mxfp4 mode: the layers' gradients land in the flat bucket that the ranks reduce.  Two
+    ranks' halves of a batch, one after the other in this process; the collective is replaced by their sum."""
+    from nerf import parallel
+    from nerf.models import NeRF, Siren
+    from nerf.rendering import render_nerf
+    torch.manual_seed(7)
+    model = {"nerf": NeRF, "siren": Siren}[tag]().to(DEV).set_training_precision("mxfp4")
+    if tag == "nerf":      # some density everywhere: an empty volume has no gradients
+        with torch.no_grad():
+            model.block2[-1].bias[model.hidden_dim] = 1.0
+    R, S = 64, 32
+    o, d = randn(R, 3, seed=5), torch.nn.functional.normalize(randn(R, 3, seed=6), dim=1)
+    tgt = torch.rand(R, 3, device=DEV, generator=torch.Generator(DEV).manual_seed(2))
+    u = torch.rand(S, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+
+    def loss(sl):
+        rgb = render_nerf(model, o[sl], d[sl], 2.0, 6.0, num_samples=S, device=DEV, u=[u])
+        return torch.nn.functional.mse_loss(rgb, tgt[sl])
+
+    shards = [parallel.shard_slice(R, r, 2) for r in range(2)]
+    want = [torch.cat([g.reshape(-1) for g in torch.autograd.grad(loss(sl), list(model.parameters()))]) for sl in shards]
+    assert float(want[0].norm()) > 0 and not torch.equal(want[0], want[1])
+    flat = parallel.FlatParameters(model)
+    buckets = []
+    for sl in shards:
+        flat.zero_grad()
+        loss(sl).backward()
+        buckets.append(flat.grad.clone())
+    monkeypatch.setattr(parallel, "world", lambda: (0, 2))
+    monkeypatch.setattr(parallel.dist, "all_reduce", lambda t, op=None: t.copy_(buckets[0] + buckets[1]))
+    flat.all_reduce_mean()
+    mean = (want[0].double() + want[1].double()) / 2
+    # the same shard twice: the kernels' sums are the same, those that atomics may reorder differ by their rounding
+    assert float((flat.grad.double() - mean).norm() / mean.norm()) < 1e-6
+    opt, before = parallel.FusedAdam(flat, lr=5e-4), flat.flat.clone()
+    opt.step()
+    assert not torch.equal(flat.flat, before) and all(p.data_ptr() >= flat.flat.data_ptr() for p in model.parameters())
