@@ -248,8 +248,9 @@ int nerf_linear_bwd_noalloc(const float* dy, int64_t lddy, const float* y, const
  * index, 16-byte aligned), scales [rows][4 ceil(K / 128)] bytes (4-byte aligned); nerf_mx_codes_bytes /
  * nerf_mx_scales_bytes give the sizes (0 for sizes the library does not take).
  * Types of x, bias, y, dy and the gradients: NERF_F32, NERF_BF16 or NERF_F16, one per call; element pitches ldx, ldy ...
- * may exceed the row length.  K up to 2^22, fewer than 2^32 groups of eight values in the padded rows; up to 2^30 rows of x in
- * a product, 65535 * 64 rows of x and of W in one that keeps its input for a backward pass. */
+ * may exceed the row length.  K up to 2^22; rows times 16 ceil(K / 128), their groups of eight values, at most 2^32 - 256 (so
+ * fewer than 2^28 rows at any K).  A product takes up to 2^22 rows of W and fewer than 2^24 tiles of 128 x 128 in y; one that
+ * keeps its input for a backward pass 65535 * 64 rows of x and of W. */
 #define NERF_F32 0
 #define NERF_BF16 1
 #define NERF_F16 2

@@ -140,8 +140,8 @@ __device__ __forceinline__ bf16x8 read_turned(const uint8_t* __restrict__ at, in
 }
 
 
-// what every entry point checks of its sizes: 32-bit offsets inside a tile of 256 rows, int row counts of weights
-// K up to 2^22; a thread for every eight values of the padded rows, less than 2^32 in a launch
+// What every entry point checks of its sizes.  K up to 2^22: 32-bit offsets inside a tile of 256 rows.  A thread for every eight
+// values of the padded rows, whole workgroups of them below 2^32 in a launch: with K <= 128 that is fewer than 2^28 rows.
 static inline bool sizes_ok(int64_t rows, int64_t K) {
     return rows >= 0 && K >= 1 && K <= (1 << 22) && rows <= 0xffffff00ll / (code_pitch(K) / 4);
 }

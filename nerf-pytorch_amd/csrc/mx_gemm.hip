@@ -938,10 +938,10 @@ int backward(const char* fn, const BwdLayout& l, DzArgs dz, const uint8_t* xcode
 
 using namespace mxk;
 
-// M up to 2^30 rows, K and N up to 2^22: 32-bit offsets inside a tile, int tile counts
+// On top of what the packed rows ask (fewer than 2^28 of them): an int N that 32-bit offsets reach, and a launch of fewer than
+// 2^32 threads
 static bool linear_sizes_ok(int64_t M, int64_t K, int64_t N) {
-    return M >= 0 && M <= (1 << 30) && sizes_ok(M, K) && N >= 1 && N <= (1 << 22) && sizes_ok(N, K) &&
-           ceil_div64(M, 128) * ceil_div64(N, 128) < (1 << 24);   // 2^32 threads in a launch
+    return sizes_ok(M, K) && N >= 1 && N <= (1 << 22) && sizes_ok(N, K) && ceil_div64(M, 128) * ceil_div64(N, 128) < (1 << 24);
 }
 
 constexpr int64_t kTrainRows = 65535ll * 64;   // of a backward pass: grid.y; 32-bit offsets inside a turned tile

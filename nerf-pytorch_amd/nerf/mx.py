@@ -13,7 +13,8 @@ holds a NaN or an infinity stands for NaN as a whole.
 
 All of them run on the current stream of the tensors' device, allocate their outputs and workspaces from torch's allocator
 and can be captured into a graph (with gradients: torch.autograd.grad inside the capture, after a warm-up on another stream).
-K is at most 2^22; a call that trains takes up to 65535 * 64 rows of x and of the weight.
+K is at most 2^22 and a matrix of packed rows below 2^32 groups of eight values (rows * 16 * ceil(K / 128)); a product takes
+weights of up to 2^22 rows, a call that trains up to 65535 * 64 rows of x and of the weight.
 """
 from __future__ import annotations
 

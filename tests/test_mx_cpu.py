@@ -214,3 +214,28 @@ def test_large_tile_reads_its_scales_inside_lds(tmp_path):
     subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", "-o", str(exe), source], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True)
     assert out.returncode == 0, out.stdout
+
+
+@pytest.mark.parametrize("K, rows", [(1, 268435440), (128, 268435440), (129, 134217720), (1 << 22, 8191)])
+def test_most_rows_that_are_taken(K, rows):
+    """rows * 16 ceil(K / 128) groups of eight values, at most 2^32 - 256: accepted up to there (a NULL pointer is all that is
+    wrong then), refused behind."""
+    from nerf import _hip
+    lib = _hip.lib
+    assert rows * 16 * -(-K // 128) <= 2 ** 32 - 256 < (rows + 1) * 16 * -(-K // 128)
+    assert lib.nerf_mx_codes_bytes(rows, K) == rows * 64 * -(-K // 128) and lib.nerf_mx_codes_bytes(rows + 1, K) == 0
+    assert lib.nerf_mx_scales_bytes(rows, K) == rows * 4 * -(-K // 128) and lib.nerf_mx_scales_bytes(rows + 1, K) == 0
+    assert lib.nerf_mx_quantize(None, 0, K, rows, K, P, P, None) == -2
+    assert lib.nerf_mx_quantize(None, 0, K, rows + 1, K, P, P, None) == -1
+    assert lib.nerf_mx_linear_fwd(*_fwd(M=rows, K=K, ldx=K, x=None)) == -2
+    assert lib.nerf_mx_linear_fwd(*_fwd(M=rows + 1, K=K, ldx=K, x=None)) == -1 and b"bad shape" in lib.nerf_last_error()
+
+
+def test_most_outputs_that_are_taken():
+    """Up to 2^22 rows of W and fewer than 2^24 tiles of 128 x 128 in y."""
+    from nerf import _hip
+    lib, n = _hip.lib, 1 << 22
+    assert lib.nerf_mx_linear_fwd(*_fwd(N=n, ldy=n, x=None)) == -2
+    assert lib.nerf_mx_linear_fwd(*_fwd(N=n + 1, ldy=n + 1, x=None)) == -1 and b"bad shape" in lib.nerf_last_error()
+    assert lib.nerf_mx_linear_fwd(*_fwd(M=128 * 511, N=n, ldy=n, x=None)) == -2
+    assert lib.nerf_mx_linear_fwd(*_fwd(M=128 * 511 + 1, N=n, ldy=n, x=None)) == -1 and b"bad shape" in lib.nerf_last_error()
