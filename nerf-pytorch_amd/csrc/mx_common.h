@@ -1,5 +1,5 @@
-// Shared pieces of the microscaled 4-bit (MXFP4) operators: mx.hip (quantise, read back, single-token product),
-// mx_gemm.hip (tiled products, gradients).
+// Shared pieces of the microscaled 4-bit (MXFP4) operators: mx.hip (quantise, read back), mx_few.hip (products with few rows),
+// mx_narrow.hip (narrow layers over many rows, forward and backward), mx_gemm.hip (tiled products, the other gradients).
 //
 // The format.  A row is cut into blocks of 32 values.  A block holds one scale byte s, standing for 2^(s - 127), and 32
 // codes of 4 bits (sign, two exponent bits, one mantissa bit): 0 .5 1 1.5 2 3 4 6.  With E the biased fp32 exponent

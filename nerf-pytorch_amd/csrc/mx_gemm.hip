@@ -320,7 +320,7 @@ __device__ __forceinline__ void settle_all(f32x4 (&acc)[NI][MI]) {
 // and the matrix instruction picks the byte.  Scales are requested for two stages at a time, 16 bytes a row (8-byte
 // requests of 512 rows cost the L2 as much as the codes did); the last window of a row is moved back to end with it.  LDS serves
 // sixteen lanes at a time, of two neighbouring groups: with q and q + 1 in places 2q and 2q + 2 the permutation of a row is
-// another than for bf16 (half of the LDS cycles were conflicts before, 138 -> 135 us).
+// another than for bf16 (half of the LDS cycles were conflicts before, 138 -> 135 us; 17 % are left, 2.0 of 12.1 M; bf16 has none).
 //
 // Rows of 64 bytes a stage in a ring of four were slower: requests of half a cache line halve what the L2 delivers.
 template <int KIND, typename T, int ACT>
@@ -544,7 +544,8 @@ __global__ __launch_bounds__(256) void mx_finish_kernel(Finish f, int64_t M, int
 // the weight gradient (either may be NULL); Np, Mp: rounded up to 64, zeros behind the end.  colsum: partial column sums
 // of dz [grid.y][N], or NULL.  Tiles of 64 x 64, `deep` of them one under the other per workgroup; the terms go through LDS
 // as rows and are read out turned.  Bound by bytes, and by launch and latency where there are few: 4096 x 4096 bf16, whose rows
-// the product reads in place, 67 MB in 18 us; 6000 x 257 fp32 with slopes 33 MB in 13 us.
+// the product reads in place, 67 MB in 18 us; 6000 x 257 fp32 with slopes 33 MB in 13 us.  16 to 20 % of the LDS cycles are bank
+// conflicts.
 struct DzArgs {
     const void* dy;
     int64_t lddy;
@@ -685,7 +686,8 @@ __global__ __launch_bounds__(256) void mx_colsum_kernel(const float* __restrict_
 }
 
 // Packed rows [rows][K] -> turned bf16 values [K][rows_p], zeros behind the last row.  Tiles of 64 rows x 128 values; W and x
-// in one launch, neighbouring workgroups write neighbours.  Bound by bytes: 4096 x 4096 both, 86 MB in 16 us.
+// in one launch, neighbouring workgroups write neighbours.  Bound by bytes: 4096 x 4096 both, 86 MB in 16 us; half of its LDS
+// cycles are bank conflicts, of rows eight apart that start on the same bank.
 struct Turn {
     const uint8_t *codes, *scales;
     int64_t rows, rows_p;       // rows_p: 0 where there is nothing to turn
@@ -733,9 +735,13 @@ struct Plan {
 
 // Tile and split of an M x N product over rows of `steps` times 64 bytes.
 //
-// The largest tile that leaves no compute unit idle: a tile of 256 x 256 reads half of what 128 x 128 does for each product,
-// and a quarter of idle units is less than that (rounding and packed product in bf16, tiles of 128 against 256: 4096 x 4096 ->
-// 4096 70 : 54 us, 4096 x 8192 -> 8192 198 : 150, 3328 x 4096 -> 4096, 208 tiles, 60 : 47, 16384 x 1024 -> 1024 34 : 30).  Below
+// The largest tile of which there are three for every four compute units, counting tiles at the edges as whole ones: a tile of
+// 256 x 256 reads half of what 128 x 128 does for each product, and a quarter of idle units is less than that (rounding and packed
+// product in bf16, tiles of 128 against 256: 4096 x 4096 -> 4096 70 : 54 us, 4096 x 8192 -> 8192 198 : 150, 3328 x 4096 -> 4096, 208
+// tiles, 60 : 47, 16384 x 1024 -> 1024 34 : 30).  Little is lost where tiles are wide of what they cover or start a second
+// round: tiles of 64 : 128 : 256, rounding and product in bf16, 50000 x 1000 -> 16 31 : 35 : 37 us, -> 64 32 : 35 : 38, -> 130 40 : 44 :
+// 38, 32768 x 4096 -> 257 111 : 104 : 103, 4096 x 4096 -> 4352, 272 tiles, 92 : 78 : 77, -> 4608 99 : 78 : 77; fp32 data gradient of
+// 32 -> 2000 over 50000 rows 406 : 397 : 420, of 130 -> 2000 504 : 475 : 427.  Below
 // 256 tiles of 128 the work goes to tiles of 64 (1024^3 training in bf16 66 -> 53 us, 512 x 4096 -> 4096 32 -> 23.6 us, rows of
 // 319 -> 257 over 6000 in fp32 86 -> 74 us), and where those are too few the reduction is split.
 Plan plan_for(int64_t M, int64_t N, int64_t steps, int terms) {

@@ -9,7 +9,8 @@ constexpr int kNarrow = 256;            // inputs and outputs
 // Against the general way, us: forward 256 -> 256 relu fp32 with 8192 rows 11.3 : 8.1, 16384 13.3 : 14.1; sin fp32 with 12288
 // 16.2 : 10.7, 16384 16.7 : 17.2, 32768 21.4 : 22.5; 64 -> 64 sin fp32 with 32768 8.6 : 15.5.  Backward 256 -> 256 sin fp32 with
 // 4096 39.9 : 40.1, 8192 44.4 : 48.6, 32768 57 : 117, relu bf16 with 4096 31.0 : 28.3, 8192 36.0 : 35.3, 32768 47 : 63; 64 -> 64
-// sin fp32 with 4096 18.0 : 23.2.
+// sin fp32 with 4096 18.0 : 23.2.  The borders are those of 256 columns; narrower layers cross earlier, as the figures of 64 show,
+// and take the general way for longer than they need.
 constexpr int64_t kNarrowRowsFwd = 16384, kNarrowRowsBwd = 4096;
 
 struct NarrowFwd {
