@@ -260,3 +260,113 @@ def test_flat_bucket_holds_the_mean_over_ranks(tag, monkeypatch):
     opt, before = parallel.FusedAdam(flat, lr=5e-4), flat.flat.clone()
     opt.step()
     assert not torch.equal(flat.flat, before) and all(p.data_ptr() >= flat.flat.data_ptr() for p in model.parameters())
+
+
+# ---------------------------------------------------------------------------------------------------- the ends of the sizes
+def whole(*shape, seed):
+    """-1, 0 and 1: exact in every block, and sums of up to 2^24 of their products are exact in fp32 in any order."""
+    g = torch.Generator(DEV).manual_seed(seed)
+    return torch.randint(-1, 2, shape, generator=g, device=DEV, dtype=torch.int8).float()
+
+
+def product64(a, b):
+    """a [m,k] b [n,k]^T in float64, a piece of k at a time."""
+    out = torch.zeros(a.shape[0], b.shape[0], dtype=torch.float64, device=DEV)
+    for k in range(0, a.shape[1], 1 << 18):
+        out += a[:, k:k + (1 << 18)].double() @ b[:, k:k + (1 << 18)].double().t().contiguous()
+    return out
+
+
+@pytest.mark.parametrize("M, K, N", [(3, 1 << 22, 17), (40, 1 << 22, 17), (40, (1 << 22) - 129, 9)])
+def test_longest_rows(M, K, N):
+    x, w, b, dy = whole(M, K, seed=1), whole(N, K, seed=2), whole(N, seed=3), whole(M, N, seed=4)
+    y, (dx, dw, db) = run_training(x, w, b, dy, "none")
+    assert torch.equal(y.double(), product64(x, w) + b.double())
+    assert torch.equal(dx, dy @ w) and torch.equal(dw, dy.t().contiguous() @ x) and torch.equal(db, dy.sum(0))
+
+
+def test_most_rows_of_a_weight():
+    from nerf import mx
+    for M, K, N in ((1, 40, 1 << 22), (130, 40, 1 << 22)):
+        x, w = whole(M, K, seed=1), whole(N, K, seed=2)
+        y = mx.linear(x, w)
+        for n in range(0, N, 1 << 20):
+            assert torch.equal(y[:, n:n + (1 << 20)], x @ w[n:n + (1 << 20)].t().contiguous())
+        del y
+    M, K, N = 5, 33, 65535 * 64
+    x, w, b, dy = whole(M, K, seed=1), whole(N, K, seed=2), whole(N, seed=3), whole(M, N, seed=4)
+    y, (dx, dw, db) = run_training(x, w, b, dy, "none")
+    assert torch.equal(y, x @ w.t().contiguous() + b) and torch.equal(dx.double(), product64(dy, w.t().contiguous()))
+    assert torch.equal(dw, dy.t().contiguous() @ x) and torch.equal(db, dy.sum(0))
+
+
+def test_most_rows():
+    """2^28 - 16 rows: rounded, read back and multiplied."""
+    from nerf import mx
+    rows = 268435440
+    x = whole(rows, 1, seed=1)
+    q = mx.quantize(x)
+    assert torch.equal(mx.dequantize(q), x)
+    del q
+    w, b = torch.full((1, 1), 2.0, device=DEV), torch.ones(1, device=DEV)
+    y = mx.linear(x, w, b, mx.ACT_RELU)
+    assert torch.equal(y, torch.relu(2 * x + 1))
+
+
+# ------------------------------------------------------------------------------------------------------------- calls in turn
+@pytest.mark.parametrize("act", ACTS)
+def test_backward_twice_and_after_other_calls(act):
+    """What a forward keeps is its own: other layers' calls in between and a second backward change nothing."""
+    from nerf import mx
+    cases = [training_case(M, K, N, act, torch.float32) for M, K, N in ((30, 200, 72), (700, 200, 72), (4200, 200, 72))]
+    want = [run_training(*c, act) for c in cases]
+    runs = []
+    for x, w, b, dy in cases:
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        runs.append((mx.linear(*leaves, mx.ACTIVATIONS[act]), leaves, dy))
+    for _ in range(2):
+        for (y, leaves, dy), (wy, wg) in list(zip(runs, want))[::-1]:
+            got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+            assert torch.equal(y, wy) and all(torch.equal(a, c) for a, c in zip(got, wg))
+
+
+def test_two_threads():
+    """Two host threads, each on a stream of its own."""
+    import threading
+    cases = [training_case(M, K, N, "sin", torch.float32) for M, K, N in ((20, 300, 72), (700, 256, 256), (5000, 200, 72), (3400, 300, 3601))]
+    want = [run_training(*c, "sin") for c in cases]
+    torch.cuda.synchronize()
+    results = {}
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            results[k] = [[run_training(*c, "sin") for c in cases[::1 if k else -1]][::1 if k else -1] for _ in range(3)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for k in range(2):
+        for run in results[k]:
+            for a, c in zip(run, want):
+                assert torch.equal(a[0], c[0]) and all(torch.equal(g, h) for g, h in zip(a[1], c[1]))
+
+
+@pytest.mark.parametrize("tag", ["nerf", "siren"])
+def test_gradients_of_the_points_alone(tag):
+    """A frozen network in the mxfp4 mode: the same outputs as without gradients, and d out / d points from the layers' dx."""
+    from nerf.models import NeRF, Siren
+    torch.manual_seed(3)
+    model = {"nerf": NeRF, "siren": Siren}[tag]().to(DEV).set_inference_precision("mxfp4")
+    if tag == "nerf":
+        with torch.no_grad():
+            model.block2[-1].bias[model.hidden_dim] = 1.0
+    model.requires_grad_(False)
+    pts, dirs = randn(5000, 3, seed=1, scale=0.4), torch.nn.functional.normalize(randn(5000, 3, seed=2), dim=1)
+    with torch.no_grad():
+        c, d = model(pts, dirs)
+    leaf = pts.clone().requires_grad_(True)
+    ce, de = model(leaf, dirs)
+    assert torch.equal(c, ce) and torch.equal(d, de)
+    (g,) = torch.autograd.grad(ce.sum() + de.sum(), leaf)
+    assert torch.isfinite(g).all() and float(g.abs().max()) > 0
