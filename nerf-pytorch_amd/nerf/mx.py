@@ -12,7 +12,9 @@ holds a NaN or an infinity stands for NaN as a whole.
     w = mx.dequantize(q, torch.bfloat16)    # the values the codes stand for
 
 All of them run on the current stream of the tensors' device, allocate their outputs and workspaces from torch's allocator
-and can be captured into a graph (with gradients: torch.autograd.grad inside the capture, after a warm-up on another stream).
+and can be captured into a graph (with gradients: torch.autograd.grad inside the capture, after a warm-up on another stream, and
+with no result of an eager pass over the same leaves still alive: it holds the leaves' autograd nodes on the eager stream, and a
+capture that has to wait for that ends the process).
 K is at most 2^22 and a matrix of packed rows below 2^32 groups of eight values (rows * 16 * ceil(K / 128)); a product takes
 weights of up to 2^22 rows, a call that trains up to 65535 * 64 rows of x and of the weight.
 """
